@@ -74,6 +74,11 @@ SYMBOLS = {
     "b200p_gemm_16": (_i, [_i, _i, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _vp]),
     "b200p_session_graph_replays": (C.c_ulonglong, [_vp]),
     "b200p_session_mega_launches": (C.c_ulonglong, [_vp]),
+    "b200p_attn_prefill_packed_workspace_bytes": (_sz, [_vp]),
+    "b200p_attn_prefill_packed": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "b200p_attn_decode_shared_workspace_bytes": (_sz, [_vp]),
+    "b200p_attn_decode_shared": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "b200p_logits_adjust": (_i, [_vp, _vp, _vp, _vp]),
     "b200p_fa_step": (_i, [_i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, C.c_float, _vp]),
 }
 
@@ -519,6 +524,217 @@ def fa_rows_f32(variant: str, bc: int, Q, K, V, scale: float = 0.0, out=None):
         out = torch.empty_like(Q)
     _check(lib().b200p_fa_rows_f32({"naive": 0, "dpp": 1}[variant], bc, Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr(),
                                    batch, heads, seq, D, float(scale), _stream(Q)), "fa_rows_f32")
+    return out
+
+
+# ---- a batch of requests of different lengths -----------------------------------------------------
+class PackedArgs(C.Structure):
+    """struct b200p_packed_args (include/b200p.h)."""
+    _fields_ = [(n, _i) for n in ("D", "nQHeads", "nKVHeads", "batch", "total_q", "total_k", "causal", "dtype")] + [("scale", C.c_float)] + [
+        (n, _ll) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "o_token", "o_head")]
+
+
+class SharedArgs(C.Structure):
+    """struct b200p_shared_args (include/b200p.h)."""
+    _fields_ = [(n, _i) for n in ("D", "nQHeads", "nKVHeads", "batch", "prefix_len", "max_own", "dtype")] + [("scale", C.c_float)] + [
+        (n, _ll) for n in ("prefix_head", "own_head", "own_batch", "q_batch", "o_batch")]
+
+
+class LogitsArgs(C.Structure):
+    """struct b200p_logits_args (include/b200p.h)."""
+    _fields_ = [(n, _i) for n in ("dtype", "rows", "vocab", "prompt_max", "tokens_max", "bias_n", "n_masks")] + [
+        (n, _ll) for n in ("in_stride", "out_stride")] + [
+        (n, _vp) for n in ("prompt", "prompt_lengths", "tokens", "token_lengths", "repetition", "presence", "frequency", "bias_ids", "bias_values", "mask", "mask_rows")]
+
+
+def _together(first, tensors, ints=()):
+    """Checks a call's tensors: all on the first one's CUDA device, of its type (`ints`: int32 and contiguous)."""
+    import torch
+    if not first.is_cuda:
+        raise ValueError("tensors must be CUDA tensors: there is no CPU path")
+    device, dtype = first.get_device(), first.dtype
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("all tensors of a call must be on one CUDA device")
+        if t.dtype != dtype:
+            raise ValueError("Q, K, V and the output must have one type")
+    for t in ints:
+        if t.get_device() != device:
+            raise ValueError("all tensors of a call must be on one CUDA device")
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError("offsets, lengths and ids must be contiguous int32 tensors")
+
+
+class _on:
+    """The tensor's device as the current one, which is what the library launches on."""
+    def __init__(self, t):
+        import torch
+        device = t.get_device()
+        self._guard = torch.cuda.device(device) if torch.cuda.current_device() != device else None
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *e):
+        if self._guard is not None:
+            self._guard.__exit__(*e)
+
+
+def _scratch(workspace, nbytes: int, like):
+    """(pointer, bytes) of the caller's workspace, or of one made for this call."""
+    import torch
+    if workspace is not None:
+        if workspace.get_device() != like.get_device() or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous tensor on the other tensors' device")
+        return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if nbytes == 0:
+        return None, None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return ws, ws.data_ptr(), nbytes
+
+
+def _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out):
+    if Q.dim() != 3 or K.dim() != 3 or K.shape != V.shape or out.shape != Q.shape or K.shape[2] != Q.shape[2]:
+        raise ValueError("Q and out are [tokens, heads, D], K and V [tokens, kv_heads, D]")
+    if q_offsets.dim() != 1 or q_offsets.shape != k_offsets.shape or q_offsets.numel() == 0:
+        raise ValueError("q_offsets and k_offsets have batch + 1 entries")
+    for t in (Q, K, V, out):
+        if t.stride(2) != 1:
+            raise ValueError("the head dimension must be contiguous")
+    if str(Q.dtype) not in ("torch.float16", "torch.bfloat16"):
+        raise ValueError("Q, K and V must be fp16 or bf16")
+    return PackedArgs(Q.shape[2], Q.shape[1], K.shape[1], q_offsets.numel() - 1, Q.shape[0], K.shape[0], int(bool(causal)), _dtype_code(Q), float(scale),
+                      Q.stride(0), Q.stride(1), K.stride(0), K.stride(1), V.stride(0), V.stride(1), out.stride(0), out.stride(1))
+
+
+def prefill_packed_workspace(Q, K, V, q_offsets, k_offsets=None, causal: bool = True):
+    """Scratch tensor for prefill_packed with tensors of these shapes (it may be empty)."""
+    import torch
+    a = _packed_args(Q, K, V, q_offsets, q_offsets if k_offsets is None else k_offsets, causal, 0.0, Q)
+    with _on(Q):
+        return torch.empty(int(lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(a))), dtype=torch.uint8, device=Q.device)
+
+
+def prefill_packed(Q, K, V, q_offsets, k_offsets=None, causal: bool = True, scale: float = 0.0, out=None, workspace=None):
+    """Attention of prompts of different lengths that lie one after the other: Q [tokens, heads, D], K and V [keys, kv_heads, D]
+    (fp16 or bf16, any 8-element aligned strides); sequence b has the rows q_offsets[b] .. q_offsets[b + 1] of Q and
+    k_offsets[b] .. k_offsets[b + 1] of K and V (int32 CUDA tensors of batch + 1 entries; default: the same rows).  Causal: a sequence's
+    last query sees all its keys, each one before it sees one key less, so keys beyond the queries are a cache in front of them.  A
+    query without keys gets zeros; rows of out outside all sequences are left as they are.  scale 0: 1 / sqrt(D)."""
+    import torch
+    if k_offsets is None:
+        k_offsets = q_offsets
+    if out is None:
+        out = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
+    _together(Q, (K, V, out), (q_offsets, k_offsets))
+    a = _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out)
+    with _on(Q):
+        ws, at, n = _scratch(workspace, int(lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(a))), Q)
+        _check(lib().b200p_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), out.data_ptr(),
+                                               C.byref(a), at, n, _stream(Q)), "attn_prefill_packed")
+    return out
+
+
+def _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out):
+    if q.dim() != 3 or K_prefix.dim() != 3 or K.dim() != 4 or K_prefix.shape != V_prefix.shape or K.shape != V.shape or out.shape != q.shape:
+        raise ValueError("q and out are [batch, heads, D], the prefix [kv_heads, keys, D], K and V [batch, kv_heads, keys, D]")
+    batch, heads, D = q.shape
+    kv, room, most = K_prefix.shape[0], K_prefix.shape[1], K.shape[2]
+    if K.shape[0] != batch or K.shape[1] != kv or K.shape[3] != D or K_prefix.shape[2] != D:
+        raise ValueError("q, the prefix and the caches must agree in batch, key heads and head size")
+    n = room if prefix_len is None else int(prefix_len)
+    if not 0 <= n <= room:
+        raise ValueError(f"prefix_len must be 0 .. {room}")
+    if str(q.dtype) not in ("torch.float16", "torch.bfloat16"):
+        raise ValueError("q, K and V must be fp16 or bf16")
+    # a dimension of one element may have any stride
+    own_head, own_batch = K.stride(1) if kv > 1 else most * D, K.stride(0) if batch > 1 else kv * most * D
+    for t in (K_prefix, V_prefix, K, V):
+        if t.stride(-1) != 1 or (t.shape[-2] > 1 and t.stride(-2) != D):
+            raise ValueError("the rows of a key head must follow one another")
+    if K_prefix.stride() != V_prefix.stride() or K.stride() != V.stride():
+        raise ValueError("K and V must have the same strides")
+    for t in (q, out):
+        if t.stride(2) != 1 or (heads > 1 and t.stride(1) != D):
+            raise ValueError("the heads of q and of out must follow one another")
+    return SharedArgs(D, heads, kv, batch, n, most, _dtype_code(q), float(scale), K_prefix.stride(0) if kv > 1 else room * D, own_head, own_batch,
+                      q.stride(0) if batch > 1 else heads * D, out.stride(0) if batch > 1 else heads * D)
+
+
+def decode_shared_workspace(q, K_prefix, K, prefix_len=None):
+    """Scratch tensor for decode_shared with tensors of these shapes (it may be empty)."""
+    import torch
+    a = _shared_args(q, K_prefix, K_prefix, K, K, prefix_len, 0.0, q)
+    with _on(q):
+        return torch.empty(int(lib().b200p_attn_decode_shared_workspace_bytes(C.byref(a))), dtype=torch.uint8, device=q.device)
+
+
+def decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len=None, scale: float = 0.0, out=None, workspace=None):
+    """One new token per sequence, behind a prefix that all sequences share and that is read once for all of them: q [batch, heads, D]
+    attends to the first prefix_len keys of K_prefix / V_prefix [kv_heads, max_prefix, D] (default: all) and to the first lengths[b]
+    keys of its own cache K / V [batch, kv_heads, max_own, D].  lengths: int32 CUDA tensor, read on the device.  A sequence without
+    keys gets zeros.  scale 0: 1 / sqrt(D)."""
+    import torch
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _together(q, (K_prefix, V_prefix, K, V, out), (lengths,))
+    a = _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out)
+    if lengths.dim() != 1 or lengths.numel() != q.shape[0]:
+        raise ValueError("lengths has one entry per sequence")
+    with _on(q):
+        ws, at, n = _scratch(workspace, int(lib().b200p_attn_decode_shared_workspace_bytes(C.byref(a))), q)
+        _check(lib().b200p_attn_decode_shared(q.data_ptr(), K_prefix.data_ptr(), V_prefix.data_ptr(), K.data_ptr(), V.data_ptr(), lengths.data_ptr(),
+                                              out.data_ptr(), C.byref(a), at, n, _stream(q)), "attn_decode_shared")
+    return out
+
+
+def adjust_logits(logits, prompt=None, prompt_lengths=None, tokens=None, token_lengths=None, repetition=None, presence=None, frequency=None,
+                  bias_ids=None, bias_values=None, mask=None, mask_rows=None, out=None):
+    """The rules of each row's request on its logits [rows, vocab] (fp32, fp16 or bf16): penalties for the tokens of `prompt` and
+    `tokens` (generated so far; int32 [rows, n], with int32 lengths [rows], default all), fp32 [rows] each: repetition divides positive and multiplies
+    other logits of tokens in either, frequency times the count and presence are subtracted for generated ones; then biases
+    (ids int32, values fp32, both [rows, n]); then tokens whose bit in `mask` (int32 [masks, (vocab + 31) // 32]) is 0 become -inf, where
+    mask_rows (int32 [rows], default: row i takes mask i) names a row's mask or, with -1, none.  Ids outside the vocabulary are
+    ignored.  out may be logits itself."""
+    import torch
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if logits.dim() != 2 or out.shape != logits.shape:
+        raise ValueError("logits and out are [rows, vocab]")
+    R, V = logits.shape
+    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(logits.dtype)
+    if code is None:
+        raise ValueError("logits must be fp32, fp16 or bf16")
+    words = (V + 31) // 32
+    _together(logits, (out,), [t for t in (prompt, prompt_lengths, tokens, token_lengths, bias_ids, mask, mask_rows) if t is not None])
+    for t in (repetition, presence, frequency, bias_values):
+        if t is not None and (t.get_device() != logits.get_device() or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError("penalties and bias values must be contiguous fp32 tensors on the logits' device")
+    for t in (prompt_lengths, token_lengths, repetition, presence, frequency, mask_rows):
+        if t is not None and tuple(t.shape) != (R,):
+            raise ValueError("lengths, penalties and mask_rows have one entry per row")
+    for t in (prompt, tokens, bias_ids):
+        if t is not None and (t.dim() != 2 or t.shape[0] != R):
+            raise ValueError("prompt, tokens and bias_ids have one row per row of the logits")
+    if (bias_ids is None) != (bias_values is None) or (bias_ids is not None and bias_ids.shape != bias_values.shape):
+        raise ValueError("bias_ids and bias_values go together")
+    if (prompt is None and prompt_lengths is not None) or (tokens is None and token_lengths is not None) or (mask is None and mask_rows is not None):
+        raise ValueError("lengths need their ids, mask_rows needs a mask")
+    if mask is not None and (mask.dim() != 2 or mask.shape[1] != words or (mask_rows is None and mask.shape[0] != R)):
+        raise ValueError(f"mask is [masks, {words}], with one mask per row or mask_rows")
+    for t in (logits, out):
+        if (V > 1 and t.stride(1) != 1) or (R > 1 and t.stride(0) < V):
+            raise ValueError("the logits of a row must follow one another")
+    if R == 0 or V == 0:
+        return out
+    ptr = lambda t: t.data_ptr() if t is not None and t.numel() else None
+    width = lambda t: t.shape[1] if t is not None else 0
+    a = LogitsArgs(code, R, V, width(prompt), width(tokens), width(bias_ids), mask.shape[0] if mask is not None else 0,
+                   logits.stride(0) if R > 1 else V, out.stride(0) if R > 1 else V, ptr(prompt), ptr(prompt_lengths), ptr(tokens), ptr(token_lengths),
+                   ptr(repetition), ptr(presence), ptr(frequency), ptr(bias_ids), ptr(bias_values), ptr(mask), ptr(mask_rows))
+    with _on(logits):
+        _check(lib().b200p_logits_adjust(logits.data_ptr(), out.data_ptr(), C.byref(a), _stream(logits)), "logits_adjust")
     return out
 
 

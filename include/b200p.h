@@ -358,6 +358,116 @@ int b200p_fa_step(int step, int dtype, const void* Q, const void* K, const void*
 int b200p_fa_rows_f32(int variant, int bc, const float* Q, const float* K, const float* V, float* O,
                       int batch, int heads, int seq_len, int D, float scale, b200p_stream_t stream);
 
+/* =========================================================================
+ * A batch of requests of different lengths.  No counterpart in the reference,
+ * whose batches are equal-length sequences.
+ * ========================================================================= */
+
+/* Attention of prompts of different lengths, one after the other in one tensor.
+ * Sequence b has the query rows q_offsets[b] .. q_offsets[b+1]-1 of Q and O and
+ * the key rows k_offsets[b] .. k_offsets[b+1]-1 of K and V (device arrays of
+ * batch + 1 ints that do not decrease; read on the device, nothing waits for the
+ * host).  With n queries and m keys, causal query i sees the keys j <= m - n + i:
+ * the last query sees all, keys beyond the queries are a cache in front of them.
+ * A query that sees no key (m < n) gets zeros.  Rows of O outside all sequences
+ * are left as they are.  A key that a query does not see does not reach it,
+ * whatever it holds (NaN and infinities among it).  Offsets outside the tensors
+ * are clamped to them.
+ * D 64 or 128, 16-bit I/O, fp32 softmax and accumulation; nQHeads % nKVHeads == 0,
+ * at most 128 query heads per key head.  Strides in elements, multiples of 8. */
+typedef struct b200p_packed_args {
+    int D;
+    int nQHeads;
+    int nKVHeads;
+    int batch;                 /* sequences; empty ones (no queries, no keys) are fine    */
+    int total_q, total_k;      /* rows of Q and O, rows of K and V                        */
+    int causal;
+    int dtype;                 /* B200P_F16 or B200P_BF16                                 */
+    float scale;               /* of the scores; 0 = 1/sqrt(D)                            */
+    long long q_token, q_head; /* elements between rows and between heads, per tensor;    */
+    long long k_token, k_head; /* 0, 0 = dense [rows, heads, D]                           */
+    long long v_token, v_head;
+    long long o_token, o_head;
+} b200p_packed_args;
+
+/* Bytes of caller-owned scratch (256-byte aligned) that the call needs; may be 0. */
+size_t b200p_attn_prefill_packed_workspace_bytes(const b200p_packed_args* args);
+
+int b200p_attn_prefill_packed(const void* Q, const void* K, const void* V, const int* q_offsets, const int* k_offsets, void* O,
+                              const b200p_packed_args* args, void* workspace, size_t workspace_bytes, b200p_stream_t stream);
+
+/* Decode attention for a batch whose sequences share a prefix (a system prompt, a
+ * document, the prompt of several samples): one new token per sequence attends to
+ * the prefix_len keys of K_prefix and to the first lengths[b] keys of its own
+ * cache.  The prefix exists once and is read for the whole batch, not per sequence.
+ * q, o [batch, nQHeads, D]; K_prefix, V_prefix [nKVHeads, prefix_head / D, D];
+ * K, V [batch, nKVHeads, own_head / D, D]; lengths: device array of batch ints, each
+ * taken into 0 .. max_own, and read on the device, so that a captured launch can be replayed
+ * while they grow.  A sequence without any key gets zeros.  Cache rows past a
+ * length do not reach the result, whatever they hold. */
+typedef struct b200p_shared_args {
+    int D;                     /* head dimension: 64 or 128                               */
+    int nQHeads;
+    int nKVHeads;              /* nQHeads % nKVHeads == 0, at most 128 per key head       */
+    int batch;
+    int prefix_len;            /* keys of the prefix, may be 0                            */
+    int max_own;               /* bound of lengths[], may be 0                            */
+    int dtype;                 /* B200P_F16 or B200P_BF16                                 */
+    float scale;               /* of the scores; 0 = 1/sqrt(D)                            */
+    long long prefix_head;     /* elements between KV heads of K_prefix and V_prefix;
+                                  0 = prefix_len * D                                      */
+    long long own_head;        /* elements between KV heads of K and V; 0 = max_own * D   */
+    long long own_batch;       /* elements between sequences of K and V;
+                                  0 = nKVHeads * own_head                                 */
+    long long q_batch;         /* elements between sequences in q; 0 = nQHeads * D        */
+    long long o_batch;         /* the same in o                                           */
+} b200p_shared_args;
+
+/* Bytes of caller-owned scratch (256-byte aligned) that the call needs; may be 0. */
+size_t b200p_attn_decode_shared_workspace_bytes(const b200p_shared_args* args);
+
+int b200p_attn_decode_shared(const void* q, const void* K_prefix, const void* V_prefix, const void* K, const void* V,
+                             const int* lengths, void* o, const b200p_shared_args* args, void* workspace, size_t workspace_bytes,
+                             b200p_stream_t stream);
+
+/* Rules on logits, row by row, before a token is picked.  For token t of a row with
+ * logit x, in this order, in fp32, the result rounded once to the logits' type:
+ *   t in the prompt or generated:  x = x > 0 ? x / repetition : x * repetition
+ *   t generated c > 0 times:       x = x - frequency * c - presence
+ *   t has biases:                  x = x + (their sum, taken in the list's order)
+ *   t's bit in the mask is 0:      x = -inf
+ * prompt and tokens: [rows, prompt_max] and [rows, tokens_max] token ids, of which the
+ * first prompt_lengths[row] / token_lengths[row] count (NULL: all; a length is taken into
+ * 0 .. its maximum); ids outside 0 .. vocab-1 are ignored, in the bias lists as well.
+ * mask: n_masks rows of (vocab + 31) / 32 words, token t in bit t % 32 of word t / 32;
+ * mask_rows[row] says which of them a row takes, a value outside 0 .. n_masks-1 that it
+ * takes none; NULL: row i takes mask i.  Every pointer below may be NULL
+ * (repetition 1, presence 0, frequency 0, nothing said, no bias, no mask).
+ * out may be logits itself (with the same stride). */
+typedef struct b200p_logits_args {
+    int dtype;                 /* B200P_F32, B200P_F16 or B200P_BF16                      */
+    int rows;
+    int vocab;
+    int prompt_max, tokens_max;
+    int bias_n;                /* entries of a row's bias list, at most 1024              */
+    int n_masks;
+    long long in_stride;       /* elements between rows; 0 = vocab                        */
+    long long out_stride;
+    const int* prompt;
+    const int* prompt_lengths;
+    const int* tokens;
+    const int* token_lengths;
+    const float* repetition;   /* [rows]                                                  */
+    const float* presence;     /* [rows]                                                  */
+    const float* frequency;    /* [rows]                                                  */
+    const int* bias_ids;       /* [rows, bias_n]                                          */
+    const float* bias_values;  /* [rows, bias_n]                                          */
+    const unsigned* mask;
+    const int* mask_rows;      /* [rows]                                                  */
+} b200p_logits_args;
+
+int b200p_logits_adjust(const void* logits, void* out, const b200p_logits_args* args, b200p_stream_t stream);
+
 /* Synchronises the device and reports whether any kernel of this library
  * abandoned a bounded wait since the last clear (B200P_E_TIMEOUT) or not (0). */
 int b200p_device_status(int clear);
