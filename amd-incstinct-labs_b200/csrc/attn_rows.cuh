@@ -28,7 +28,7 @@ template <typename T, int E> __device__ __forceinline__ void load_part(const T* 
 
 // Keys 0 .. n-1 of rows K + j * k_row, V + j * v_row (each D elements) into the state.  q: this lane's columns of the query.
 template <typename T, int D>
-__device__ void attend_keys(RowState<D>& st, const float (&q)[D / 32], const T* K, const T* V, long long k_row, long long v_row, int n, float scale_log2) {
+__device__ __forceinline__ void attend_keys(RowState<D>& st, const float (&q)[D / 32], const T* K, const T* V, long long k_row, long long v_row, int n, float scale_log2) {
     constexpr int E = D / 32;
     const int lane = threadIdx.x % 32;
     #pragma unroll 4

@@ -1,52 +1,21 @@
 // ---------------------------------------------------------------------------
 // packed_prefill.cu -- attention of prompts of different lengths that lie one after the other in one tensor.
 // ---------------------------------------------------------------------------
-#include "common.cuh"
-#include "attn_rows.cuh"
-#include <cmath>
+#include "packed_launch.cuh"
 
 namespace b200p {
 namespace {
 
-constexpr int kRowWarps = 4;
-
-// The sequence that row `at` belongs to: the last one whose first row is at or before it (empty sequences share their first row
-// with the next one).
-__device__ __forceinline__ int sequence_of(const int* offsets, int batch, int at) {
-    int lo = 0, hi = batch;                       // offsets[lo] <= at < offsets[hi], or at lies outside all sequences
-    while (hi - lo > 1) { const int mid = (lo + hi) / 2; if (offsets[mid] <= at) lo = mid; else hi = mid; }
-    return lo;
-}
-
-// One warp per row of Q.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32)
-packed_rows_kernel(const b200p_packed_args a, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
-                   const int* __restrict__ q_offsets, const int* __restrict__ k_offsets, T* __restrict__ O, float scale_log2) {
-    constexpr int E = D / 32;
-    const long long id = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32, head = int(id % a.nQHeads), row = int(id / a.nQHeads);
-    if (row >= a.total_q || row < q_offsets[0] || row >= q_offsets[a.batch]) return;
-    const int b = sequence_of(q_offsets, a.batch, row);
-    const int q0 = q_offsets[b], n = q_offsets[b + 1] - q0;
-    const int k0 = min(max(k_offsets[b], 0), a.total_k), keys = min(max(k_offsets[b + 1], k0), a.total_k) - k0;
-    const int seen = a.causal ? min(keys, keys - n + (row - q0) + 1) : keys;
-    const int kvh = head / (a.nQHeads / a.nKVHeads);
-    float q[E];
-    load_part<T, E>(Q + row * a.q_token + head * a.q_head + lane * E, q);
-    RowState<D> st;
-    attend_keys<T, D>(st, q, K + k0 * a.k_token + kvh * a.k_head, V + k0 * a.v_token + kvh * a.v_head, a.k_token, a.v_token, seen, scale_log2);
-    T* o = O + row * a.o_token + head * a.o_head + lane * E;
-    for (int i = 0; i < E; ++i) o[i] = from_float<T>(seen > 0 ? st.o[i] / st.l : 0.f);
-}
-
-template <typename T, int D>
-int launch_rows(const void* Q, const void* K, const void* V, const int* qo, const int* ko, void* O, const b200p_packed_args& a, float scale_log2, cudaStream_t st) {
-    const long long warps = (long long)a.total_q * a.nQHeads, ctas = (warps + kRowWarps - 1) / kRowWarps;
-    if (ctas > 0x7fffffffLL) return B200P_E_RANGE;
-    packed_rows_kernel<T, D><<<unsigned(ctas), kRowWarps * 32, 0, st>>>(a, static_cast<const T*>(Q), static_cast<const T*>(K), static_cast<const T*>(V), qo, ko,
-                                                                      static_cast<T*>(O), scale_log2);
-    return launched();
+int launch(const void* Q, const void* K, const void* V, const int* qo, const int* ko, void* O, const b200p_packed_args& a, cudaStream_t st) {
+    PackedParams p{};
+    p.Q = Q; p.K = K; p.V = V; p.O = O; p.q_offsets = qo; p.k_offsets = ko;
+    p.seqQ = a.total_q; p.seqK = a.total_k; p.batch = a.batch; p.causal = a.causal != 0;
+    p.nQH = a.nQHeads; p.nKVH = a.nKVHeads; p.group = a.nQHeads / a.nKVHeads; p.splits = 1;
+    p.scale_log2 = 1.4426950408889634f * (a.scale > 0.f ? a.scale : 1.f / sqrtf(float(D)));
+    p.q_token = a.q_token; p.q_head = a.q_head; p.k_token = a.k_token; p.k_head = a.k_head;
+    p.v_token = a.v_token; p.v_head = a.v_head; p.o_token = a.o_token; p.o_head = a.o_head;
+    return launch_packed<T, D, false>(p, a.dtype, st);
 }
 
 // Checks what the entry points share and fills in the dense strides.
@@ -89,10 +58,7 @@ extern "C" int b200p_attn_prefill_packed(const void* Q, const void* K, const voi
     if (!Q || !O || !q_offsets || !k_offsets || (a.total_k > 0 && (!K || !V))) return B200P_E_NULL;
     if (!aligned(Q, 16) || !aligned(K, 16) || !aligned(V, 16) || !aligned(O, 16) || !aligned(q_offsets, 4) || !aligned(k_offsets, 4)) return B200P_E_ALIGN;
     if (sm_count() <= 0) return B200P_E_NO_DEVICE;
-    const float scale_log2 = 1.4426950408889634f * (a.scale > 0.f ? a.scale : 1.f / sqrtf(float(a.D)));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.dtype == B200P_F16)
-        return a.D == 128 ? launch_rows<__half, 128>(Q, K, V, q_offsets, k_offsets, O, a, scale_log2, st) : launch_rows<__half, 64>(Q, K, V, q_offsets, k_offsets, O, a, scale_log2, st);
-    return a.D == 128 ? launch_rows<__nv_bfloat16, 128>(Q, K, V, q_offsets, k_offsets, O, a, scale_log2, st)
-                      : launch_rows<__nv_bfloat16, 64>(Q, K, V, q_offsets, k_offsets, O, a, scale_log2, st);
+    if (a.dtype == B200P_F16) return a.D == 128 ? launch<__half, 128>(Q, K, V, q_offsets, k_offsets, O, a, st) : launch<__half, 64>(Q, K, V, q_offsets, k_offsets, O, a, st);
+    return a.D == 128 ? launch<__nv_bfloat16, 128>(Q, K, V, q_offsets, k_offsets, O, a, st) : launch<__nv_bfloat16, 64>(Q, K, V, q_offsets, k_offsets, O, a, st);
 }

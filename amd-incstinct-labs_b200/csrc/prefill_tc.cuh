@@ -44,6 +44,7 @@
 #include "tcgen05.cuh"
 #include "tensor_map.cuh"
 #include "mma_sync.cuh"
+#include "vec_io.cuh"
 #include <type_traits>
 
 namespace b200p {
@@ -78,19 +79,31 @@ template <int QKS, int VS, int KST, int VST, int OCOLS> struct PrefillTiles {
     static constexpr int SMEM_BYTES = OFF_BAR + 1024;
     static_assert(SMEM_BYTES <= 232448, "more than an SM has");
 };
+struct PrefillParams;
+struct PackedParams;
 template <int D> struct PrefillShape : PrefillTiles<D / 64, D / 64, (D == 128) ? 2 : 4, (D == 128) ? 2 : 4, 64> {
-    static constexpr bool LATENT = false, PORTION = false, MASKED = false;
+    static constexpr bool LATENT = false, PORTION = false, MASKED = false, PACKED = false, PARTIAL = false;
+    using Params = PrefillParams;
+};
+// PACKED: sequences of different lengths, one after the other in token-major tensors (packed.cuh).  A tile's rows are the heads
+// of a group of `tokens` tokens, so that the keys of a group are read once for all its heads and short sequences fill a tile.
+// PARTIAL: a tile's keys may be split between items; O, not yet divided, and the row's maximum and sum go to a workspace in fp32.
+template <int D, bool PART> struct PackedShape : PrefillTiles<D / 64, D / 64, (D == 128) ? 2 : 4, (D == 128) ? 2 : 4, 64> {
+    static constexpr bool LATENT = false, PORTION = false, MASKED = false, PACKED = true, PARTIAL = PART;
+    using Params = PackedParams;
 };
 // PORTION: causal with an offset (a portion of a prompt starts behind the cached tokens), value columns that need not fill
 // their boxes, an optional sink in the softmax.  MASKED: a row also has a first key (AttnMask), key tiles before the first
 // row's are skipped.  Grouped heads, keys and values of different widths (grouped_attn.cuh).
 template <int QKS, int VS> struct MaskedPrefillShape : PrefillTiles<QKS, VS, (QKS + VS > 2) ? 2 : 4, (QKS + VS > 2) ? 2 : 4, 64> {
-    static constexpr bool LATENT = false, PORTION = true, MASKED = true;
+    static constexpr bool LATENT = false, PORTION = true, MASKED = true, PACKED = false, PARTIAL = false;
+    using Params = PrefillParams;
 };
 // Latent attention on expanded keys and values (latent.cuh): PLAIN boxes of a query / key row without positions, then
 // one box of the rotated part, which has its own tensor maps (the key's is the same for all heads).
 template <int PLAIN, int VS> struct LatentPrefillShape : PrefillTiles<PLAIN + 1, VS, (PLAIN + VS > 2) ? 1 : 2, 2, 32> {
-    static constexpr bool LATENT = true, PORTION = true, MASKED = false;
+    static constexpr bool LATENT = true, PORTION = true, MASKED = false, PACKED = false, PARTIAL = false;
+    using Params = PrefillParams;
 };
 
 struct PrefillParams {
@@ -144,14 +157,18 @@ __device__ __forceinline__ PrefillItem prefill_item(const PrefillParams& p, int 
     return w;
 }
 
+} // namespace b200p
+#include "packed.cuh"           // uses what is above
+namespace b200p {
+
 template <typename T, typename Sh, int RS, bool DBG>
 __global__ void __launch_bounds__(prefill_threads(RS), 1)
-prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap mapQ,
+prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorMap mapQ,
                   const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   const __grid_constant__ CUtensorMap mapO, const __grid_constant__ CUtensorMap mapQr,
                   const __grid_constant__ CUtensorMap mapKr) {
     constexpr int DV = Sh::DV;
-    constexpr bool LATENT = Sh::LATENT, PORTION = Sh::PORTION, MASKED = Sh::MASKED;
+    constexpr bool LATENT = Sh::LATENT, PORTION = Sh::PORTION, MASKED = Sh::MASKED, PACKED = Sh::PACKED, PARTIAL = Sh::PARTIAL;
     constexpr int KST = Sh::KSTAGES, VST = Sh::VSTAGES;
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::OFF_BAR);
@@ -170,9 +187,12 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_failed;
     __shared__ int s_item[2];
+    using Item = std::conditional_t<PACKED, PackedItem, PrefillItem>;
+    __shared__ std::conditional_t<PACKED, PackedItem, int> s_packed[2];
 
-    constexpr int kMmaWarp = 8 * RS, kTmaWarp = 8 * RS + 1;
-    constexpr int kItemReaders = 2 * kBM + 1;                  // every softmax thread + the MMA thread
+    constexpr int kMmaWarp = 8 * RS, kTmaWarp = 8 * RS + 1, kWalkWarp = 8 * RS + 2;
+    constexpr int kItemReaders = 2 * kBM + 1 + PACKED;         // every softmax thread + the MMA thread; PACKED: + the TMA thread
+    if constexpr (PARTIAL) griddep_launch_dependents();        // the merge that follows may get ready
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
@@ -199,9 +219,19 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
     // order a hardware block scheduler would have used) and publishes them through a two-slot ring; the
     // other roles read them there.  All barrier phases run on across items, so the next item's Q, K_0 and
     // first Q.K^T are under way while the softmax warps still normalise and store the previous item's O.
-    auto next_item = [&](int it) -> int {                      // consumer side: id of the CTA's it-th item, or -1
-        if (!dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), p.status)) return -2;
-        const int id = *reinterpret_cast<volatile int*>(&s_item[it & 1]);
+    // PACKED: a warp of its own (kWalkWarp) finds the items from the sequences' lengths, which are known on the device only, and
+    // publishes them whole; a CTA's items are a fixed share of the launch's, heaviest first, so no counter has to be cleared.
+    int* const abort_word = [&] { if constexpr (PACKED) return &s_failed; else return p.status; }();     // PACKED: no CTA waits for another
+    auto read_item = [&](int it, Item& w) -> int {             // behind item_full: the CTA's it-th item; its id, or negative: there are no more
+        if constexpr (PACKED) { w = s_packed[it & 1]; return w.kvh; }
+        else {
+            const int id = *reinterpret_cast<volatile int*>(&s_item[it & 1]);
+            return id;
+        }
+    };
+    auto next_item = [&](int it, Item& w) -> int {             // consumer side
+        if (!dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word)) return -2;
+        const int id = read_item(it, w);
         dme::mbar_arrive(&item_empty[it & 1]);
         return id;
     };
@@ -219,9 +249,18 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
         if (lane == 0) {
             dme::prefetch_tensor_map(&mapQ); dme::prefetch_tensor_map(&mapK); dme::prefetch_tensor_map(&mapV);
             dme::Ring<KST> kr; dme::Ring<VST> vr;
-            int kloads = 0, vloads = 0;
+            int kloads = 0, vloads = 0, worked = 0;
             bool ok = true;
             for (int it = 0; ok; ++it) {
+                Item w;
+                if constexpr (PACKED) {
+                    const int id = next_item(it, w);
+                    if (id < 0) { ok = id != -2; break; }
+                    if (w.nmax == 0) continue;                   // rows without keys: only zeros to write
+                    if (worked >= 1 && !dme::wait(q_empty, uint32_t((worked - 1) & 1), abort_word)) { ok = false; break; }
+                    ++worked;
+                    dme::mbar_arrive_expect_tx(q_full, uint32_t((w.n[0] > 0) + (w.n[1] > 0)) * Sh::QK_SUB * uint32_t(p.tokens * p.group) * 128u);
+                } else {
                 // draw and publish the item
                 if (it >= 2 && !dme::wait(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1), p.status)) { ok = false; break; }
                 int id = it == 0 ? int(blockIdx.x) : int(gridDim.x) + atomicAdd(p.work_counter, 1);
@@ -229,29 +268,35 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
                 s_item[it & 1] = id;
                 dme::mbar_arrive(&item_full[it & 1]);
                 if (id < 0) break;
-                const PrefillItem w = prefill_item<Sh>(p, id);
+                w = prefill_item<Sh>(p, id);
                 // Q: the previous item's last Q.K^T must be done with the buffer
                 if (it >= 1 && !dme::wait(q_empty, uint32_t((it - 1) & 1), p.status)) { ok = false; break; }
                 dme::mbar_arrive_expect_tx(q_full, uint32_t((w.n[0] > 0) + (w.n[1] > 0)) * Sh::QK_BYTES);
+                }
                 for (int t = 0; t < 2; ++t) if (w.n[t] > 0)
                     for (int sb = 0; sb < Sh::QK_SUB; ++sb) {
                         unsigned char* dst = smem + Sh::OFF_Q + t * Sh::QK_BYTES + sb * Sh::SUB_BYTES;
-                        if (LATENT && sb == Sh::QK_SUB - 1) dme::copy_tile_4d(dst, &mapQr, 0, w.q0[t], w.head, w.b, q_full);
-                        else                                dme::copy_tile_4d(dst, &mapQ, sb * 64, w.q0[t], w.head, w.b, q_full);
+                        if constexpr (LATENT) if (sb == Sh::QK_SUB - 1) { dme::copy_tile_4d(dst, &mapQr, 0, w.q0[t], w.head, w.b, q_full); continue; }
+                        if constexpr (PACKED) dme::copy_tile_4d(dst, &mapQ, sb * 64, 0, w.q_row + w.q0[t], w.kvh, q_full);
+                        else                  dme::copy_tile_4d(dst, &mapQ, sb * 64, w.q0[t], w.head, w.b, q_full);
                     }
                 for (int j = 0; j < w.nmax; ++j) {
-                    if (kloads >= KST && !dme::wait(&k_empty[kr.stage], kr.phase ^ 1u, p.status)) { ok = false; break; }
+                    if (kloads >= KST && !dme::wait(&k_empty[kr.stage], kr.phase ^ 1u, abort_word)) { ok = false; break; }
                     dme::mbar_arrive_expect_tx(&k_full[kr.stage], Sh::QK_BYTES);
                     for (int sb = 0; sb < Sh::QK_SUB; ++sb) {
                         unsigned char* dst = smem + Sh::OFF_K + kr.stage * Sh::QK_BYTES + sb * Sh::SUB_BYTES;
-                        if (LATENT && sb == Sh::QK_SUB - 1) dme::copy_tile_4d(dst, &mapKr, 0, (w.first + j) * kBN, 0, w.b, &k_full[kr.stage]);
-                        else                                dme::copy_tile_4d(dst, &mapK, sb * 64, (w.first + j) * kBN, w.kvh, w.b, &k_full[kr.stage]);
+                        if constexpr (LATENT) if (sb == Sh::QK_SUB - 1) { dme::copy_tile_4d(dst, &mapKr, 0, (w.first + j) * kBN, 0, w.b, &k_full[kr.stage]); continue; }
+                        if constexpr (PACKED) dme::copy_tile_4d(dst, &mapK, sb * 64, w.k_row + (w.first + j) * kBN, w.kvh, 0, &k_full[kr.stage]);
+                        else                  dme::copy_tile_4d(dst, &mapK, sb * 64, (w.first + j) * kBN, w.kvh, w.b, &k_full[kr.stage]);
                     }
                     kr.advance(); ++kloads;
-                    if (vloads >= VST && !dme::wait(&v_empty[vr.stage], vr.phase ^ 1u, p.status)) { ok = false; break; }
+                    if (vloads >= VST && !dme::wait(&v_empty[vr.stage], vr.phase ^ 1u, abort_word)) { ok = false; break; }
                     dme::mbar_arrive_expect_tx(&v_full[vr.stage], Sh::V_BYTES);
-                    for (int sb = 0; sb < Sh::V_SUB; ++sb)
-                        dme::copy_tile_4d(smem + Sh::OFF_V + vr.stage * Sh::V_BYTES + sb * Sh::SUB_BYTES, &mapV, sb * 64, (w.first + j) * kBN, w.kvh, w.b, &v_full[vr.stage]);
+                    for (int sb = 0; sb < Sh::V_SUB; ++sb) {
+                        unsigned char* dst = smem + Sh::OFF_V + vr.stage * Sh::V_BYTES + sb * Sh::SUB_BYTES;
+                        if constexpr (PACKED) dme::copy_tile_4d(dst, &mapV, sb * 64, w.k_row + (w.first + j) * kBN, w.kvh, 0, &v_full[vr.stage]);
+                        else                  dme::copy_tile_4d(dst, &mapV, sb * 64, (w.first + j) * kBN, w.kvh, w.b, &v_full[vr.stage]);
+                    }
                     vr.advance(); ++vloads;
                 }
             }
@@ -270,7 +315,7 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
         const uint64_t k_base = tc::smem_desc_sw128(sm_k, 16, 1024);
         const uint64_t v_base = tc::smem_desc_sw128(sm_v, Sh::SUB_BYTES, 1024);
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, dme::wait(bar, parity, p.status)) != 0; };
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, dme::wait(bar, parity, abort_word)) != 0; };
         auto issue_qk = [&](int t, int kstage) {
             const uint64_t qd = q_base + uint64_t((t * Sh::QK_BYTES) >> 4);
             const uint64_t kd = k_base + uint64_t((kstage * Sh::QK_BYTES) >> 4);
@@ -290,16 +335,24 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
         dme::Ring<KST> kr; dme::Ring<VST> vr;
         int cs0 = 0, cs1 = 0;          // steps of tile 0 / 1 in earlier items: phase of s_full / p_half
         int co0 = 0, co1 = 0;          // earlier items in which the tile had work: phase of o_done / o_free
+        int worked = 0;                // PACKED: earlier items with keys: phase of q_full
         bool ok = true;
         for (int it = 0; ok; ++it) {
             if (!wait(&item_full[it & 1], uint32_t((it >> 1) & 1))) { ok = false; break; }
-            const int id = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s_item[it & 1]), 0);
+            Item w;
+            const int id = __shfl_sync(0xffffffffu, read_item(it, w), 0);
+            if constexpr (PACKED) __syncwarp();                  // all lanes have read the item
             if (tc::elect_one()) dme::mbar_arrive(&item_empty[it & 1]);
             __syncwarp();
             if (id < 0) break;
-            const PrefillItem w = prefill_item<Sh>(p, id);
+            if constexpr (PACKED) {
+                w.nmax = __shfl_sync(0xffffffffu, w.nmax, 0); w.n[0] = __shfl_sync(0xffffffffu, w.n[0], 0); w.n[1] = __shfl_sync(0xffffffffu, w.n[1], 0);
+                w.first = __shfl_sync(0xffffffffu, w.first, 0); w.keys = __shfl_sync(0xffffffffu, w.keys, 0);
+                if (w.nmax == 0) continue;
+            } else w = prefill_item<Sh>(p, id);
             const int nmax = w.nmax, n0 = w.n[0], n1 = w.n[1];
-            ok = wait(q_full, uint32_t(it & 1)) && wait(&k_full[kr.stage], kr.phase);
+            ok = wait(q_full, uint32_t((PACKED ? worked : it) & 1)) && wait(&k_full[kr.stage], kr.phase);
+            ++worked;
             if (!ok) break;
             tc::fence_after_sync();
             if (tc::elect_one()) {
@@ -345,6 +398,18 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
                 ok = wait(&v_full[vr.stage], vr.phase);
                 if (!LATENT && ok && j + 1 < nmax) ok = wait(&k_full[kr.stage], kr.phase);
                 if (!ok) break;
+                if constexpr (PACKED) {
+                    // the rows behind the sequence's last key are another sequence's, or nobody's: their weights are 0, but a zero
+                    // times what is no number is none
+                    const int there = w.keys - (w.first + j) * kBN;
+                    if (there < kBN) {
+                        unsigned char* v = smem + Sh::OFF_V + vr.stage * Sh::V_BYTES;
+                        for (int i = lane; i < (kBN - there) * 8 * Sh::V_SUB; i += 32)      // 16 bytes at a time; the swizzle stays inside a row
+                            *reinterpret_cast<uint4*>(v + (i / ((kBN - there) * 8)) * Sh::SUB_BYTES + there * 128 + (i % ((kBN - there) * 8)) * 16) = make_uint4(0, 0, 0, 0);
+                        dme::fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
                 ok = tile_step(std::integral_constant<int, 0>{}, j, n0, cs0, co0);
                 if (ok) ok = tile_step(std::integral_constant<int, 1>{}, j, n1, cs1, co1);
                 if (!ok) break;
@@ -362,6 +427,18 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
             cs0 += n0; cs1 += n1; co0 += n0 > 0; co1 += n1 > 0;
         }
         if (!ok && lane == 0) atomicExch(&s_failed, 1);
+      } else if (PACKED && warp == kWalkWarp) {
+        if constexpr (PACKED) {
+            bool ok = true;
+            packed_walk(p, [&](int it, const PackedItem& w) -> bool {
+                if (it >= 2) ok = dme::wait(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1), abort_word);
+                ok = __all_sync(0xffffffffu, ok) != 0;
+                if (ok && lane == 0) { s_packed[it & 1] = w; dme::mbar_arrive(&item_full[it & 1]); }
+                __syncwarp();
+                return ok;
+            });
+            if (!ok && lane == 0) atomicExch(&s_failed, 1);
+        }
       }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -389,27 +466,40 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
         };
         auto tile_sync = [&]() { asm volatile("bar.sync %0, 128;" :: "r"(2 + t) : "memory"); };
         const bool issuer = r == 0;                            // issues and tracks this tile's output stores
+        int row_token = 0;                                     // PACKED: the row's token inside the tile
+        if constexpr (PACKED) row_token = r / p.group;
         unsigned char* stage = smem + Sh::OFF_OUT + t * Sh::OUT_BYTES;
         if (issuer) dme::prefetch_tensor_map(&mapO);
         for (int it = 0;; ++it) {
-          const int id = next_item(it);
+          Item w;
+          const int id = next_item(it, w);
           if (id < 0) { ok = all_of_tile(id != -2); break; }   // -1: the launch's items are used up (the same value in every thread)
-          const PrefillItem w = prefill_item<Sh>(p, id);
+          if constexpr (!PACKED) w = prefill_item<Sh>(p, id);
           const int q0t = t ? w.q0[1] : w.q0[0], nt = t ? w.n[1] : w.n[0];     // no arrays indexed at run time
-          const int o_b = w.b, o_head = w.head;
-          const int row = q0t + r;
-          const int row_pos = PORTION ? p.pos0 + row : row, q0_pos = PORTION ? p.pos0 + q0t : q0t;
+          int o_b = 0, o_head = 0;
+          if constexpr (!PACKED) { o_b = w.b; o_head = w.head; }
+          const int row = q0t + (PACKED ? row_token : r);
+          int row_pos = row, q0_pos = q0t, seqK;
+          if constexpr (PORTION) { row_pos = p.pos0 + row; q0_pos = p.pos0 + q0t; }
+          if constexpr (PACKED) { row_pos = w.ahead + row; q0_pos = w.ahead + q0t; seqK = w.keys; } else seqK = p.seqK;
+          // PACKED: whether the row is a query, and whether any of this warp's is
+          bool live = true, warp_live = true;
+          if constexpr (PACKED) { live = row_token < p.tokens && row < w.queries; warp_live = __any_sync(0xffffffffu, live); }
           const int first_key = MASKED ? p.mask.first(row_pos) : 0, last_first = MASKED ? p.mask.first(q0_pos + kBM - 1) : 0;
           float m_used = -INFINITY, l = 0.f;
           if (MASKED) { m_used = p.plus_one ? 0.f : -1e30f; l = p.plus_one ? 1.f : 0.f; }      // finite: a row may see nothing of its first tiles
-          if (PORTION && p.sink) { m_used = p.sink[o_head] * 1.4426950408889634f; l = 1.f; }    // one more term of the denominator
+          if constexpr (PORTION) if (p.sink) { m_used = p.sink[o_head] * 1.4426950408889634f; l = 1.f; }    // one more term of the denominator
           for (int j = 0; j < nt; ++j) {
-            if (!dme::wait(&s_full[t], uint32_t((cs + j) & 1), p.status)) { ok = false; break; }
+            if (!dme::wait(&s_full[t], uint32_t((cs + j) & 1), abort_word)) { ok = false; break; }
             tc::fence_after_sync();
-            const int key0 = MASKED ? (w.first + j) * kBN : j * kBN;
-            const bool need_mask = (p.causal && key0 + kBN - 1 > q0_pos) || (key0 + kBN > p.seqK) || (MASKED && key0 < last_first);
+            if (PACKED && !warp_live) {                          // O's rows of this warp are never read: any P does
+                dme::mbar_arrive(&p_half[2 * t]); dme::mbar_arrive(&p_half[2 * t + 1]);
+                continue;
+            }
+            const int key0 = MASKED || PACKED ? (w.first + j) * kBN : j * kBN;
+            const bool need_mask = (p.causal && key0 + kBN - 1 > q0_pos) || (key0 + kBN > seqK) || (MASKED && key0 < last_first);
             // columns (of this thread's range) <= col_limit are live
-            const int col_limit = min(p.causal ? row_pos : 0x7fffffff, p.seqK - 1) - key0 - half * CW;
+            const int col_limit = min(p.causal ? row_pos : 0x7fffffff, seqK - 1) - key0 - half * CW;
             const int col_first = MASKED ? first_key - key0 - half * CW : 0;
             // ---- this thread's part of the score row into registers (one wait for all loads) ------------
             uint32_t sv[CW];
@@ -478,10 +568,21 @@ prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap map
           }
           // ---- epilogue: O / l -> 16-bit, through a swizzled staging tile and TMA stores (64 columns at a time).  O is taken
           // into registers first and the tile's tensor memory released, so the next item's P.V does not wait for the stores.
-          if (ok && nt > 0) ok = dme::wait(&o_done[t], uint32_t(co & 1), p.status);
+          if (ok && nt > 0) ok = dme::wait(&o_done[t], uint32_t(co & 1), abort_word);
           ok = all_of_tile(ok);
           if (!ok) break;
-          if (nt > 0) {
+          if constexpr (PACKED) {
+            if (nt > 0) {
+                tc::fence_after_sync();
+                uint32_t v[OW];
+                #pragma unroll
+                for (int c = 0; c < OW / 32; ++c) tc::ld_32x32b_x32(tO + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
+                tc::wait_ld();
+                tc::fence_before_sync();
+                dme::mbar_arrive(&o_free[t]);
+                packed_epilogue<T, Sh>(p, w, v, m_used, l, nt, q0t, row_token, live, r, stage, issuer, tile_sync, [&](bool mine) { return !all_of_tile(!mine); }, &mapO);
+            } else if (live) packed_no_keys<T, Sh>(p, w, row, r - row_token * p.group);
+          } else if (nt > 0) {
             tc::fence_after_sync();
             uint32_t v[OW];
             #pragma unroll
