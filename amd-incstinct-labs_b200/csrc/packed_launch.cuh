@@ -8,7 +8,7 @@ namespace b200p {
 // Query tiles that all the sequences have at most, over all key heads: each may end inside one.
 inline long long packed_tiles(long long rows, int batch, int tokens, int kv_heads) { return (rows / tokens + batch) * kv_heads; }
 
-// Everything of p but the launch's own fields (tokens, span, blocks, items, sticky) is set.  k_rows: rows of K and V.
+// Everything of p but the launch's own fields (tokens, sticky; span where it is 0) is set.
 template <typename T, int D, bool PARTIAL>
 int launch_packed(PackedParams p, int dtype, cudaStream_t st) {
     using Sh = PackedShape<D, PARTIAL>;
@@ -16,7 +16,7 @@ int launch_packed(PackedParams p, int dtype, cudaStream_t st) {
     p.tokens = kBM / p.group;
     const int sms = sm_count();
     const long long tiles = packed_tiles(p.seqQ, p.batch, p.tokens, p.nKVH) * p.splits;
-    p.span = tiles <= sms ? 1 : 2;                             // a tile alone takes 0.6 of a pair's time (prefill.cu)
+    if (p.span == 0) p.span = tiles <= sms ? 1 : 2;            // a tile alone takes 0.6 of a pair's time (prefill.cu)
     const long long items = p.span == 1 ? tiles : packed_tiles(p.seqQ, p.batch, 2 * p.tokens, p.nKVH) * p.splits;
     if (items > (1 << 29)) return B200P_E_RANGE;
     CUtensorMap mq, mk, mv, mo;
