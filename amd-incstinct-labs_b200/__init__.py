@@ -547,9 +547,21 @@ class LogitsArgs(C.Structure):
         (n, _vp) for n in ("prompt", "prompt_lengths", "tokens", "token_lengths", "repetition", "presence", "frequency", "bias_ids", "bias_values", "mask", "mask_rows")]
 
 
-def _together(first, tensors, ints=()):
-    """Checks a call's tensors: all on the first one's CUDA device, of its type (`ints`: int32 and contiguous)."""
+_torch = None            # the module and what a small call asks of it, once it has been imported
+_KINDS = {}              # 16-bit types -> codes
+
+
+def _bind():
+    global _torch
     import torch
+    _KINDS.update({torch.float16: F16, torch.bfloat16: BF16})
+    _torch = torch
+    return torch
+
+
+def _together(first, tensors, ints=()):
+    """Checks a call's tensors: all on the first one's CUDA device, of its type (`ints`: int32 and contiguous).  -> the device"""
+    torch = _torch or _bind()
     if not first.is_cuda:
         raise ValueError("tensors must be CUDA tensors: there is no CPU path")
     device, dtype = first.get_device(), first.dtype
@@ -557,63 +569,53 @@ def _together(first, tensors, ints=()):
         if t.get_device() != device:
             raise ValueError("all tensors of a call must be on one CUDA device")
         if t.dtype != dtype:
-            raise ValueError("Q, K, V and the output must have one type")
+            raise ValueError("a call's Q, K, V and output, or logits and output, must have one type")
     for t in ints:
         if t.get_device() != device:
             raise ValueError("all tensors of a call must be on one CUDA device")
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError("offsets, lengths and ids must be contiguous int32 tensors")
+    return device
 
 
-class _on:
-    """The tensor's device as the current one, which is what the library launches on."""
-    def __init__(self, t):
-        import torch
-        device = t.get_device()
-        self._guard = torch.cuda.device(device) if torch.cuda.current_device() != device else None
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *e):
-        if self._guard is not None:
-            self._guard.__exit__(*e)
+def _on(device, call, *args):
+    """call(*args) with `device` as the current one, which is what the library launches on."""
+    if _torch._C._cuda_getDevice() == device:
+        return call(*args)
+    with _torch.cuda.device(device):
+        return call(*args)
 
 
-def _scratch(workspace, nbytes: int, like):
-    """(pointer, bytes) of the caller's workspace, or of one made for this call."""
-    import torch
-    if workspace is not None:
-        if workspace.get_device() != like.get_device() or not workspace.is_contiguous():
-            raise ValueError("workspace must be a contiguous tensor on the other tensors' device")
-        return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    if nbytes == 0:
-        return None, None, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    return ws, ws.data_ptr(), nbytes
+def _scratch(workspace, size, a, like, device):
+    """The caller's workspace, or one made for this call, of the size that the library asks for (or None)."""
+    if workspace is None:
+        n = _on(device, size, C.byref(a))
+        return like.new_empty(n, dtype=_torch.uint8) if n else None
+    if workspace.get_device() != device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the other tensors' device")
+    return workspace
 
 
 def _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out):
-    if Q.dim() != 3 or K.dim() != 3 or K.shape != V.shape or out.shape != Q.shape or K.shape[2] != Q.shape[2]:
+    torch = _torch or _bind()
+    qs, ks, shape = Q.shape, K.shape, q_offsets.shape
+    if len(qs) != 3 or len(ks) != 3 or ks != V.shape or out.shape != qs or ks[2] != qs[2]:
         raise ValueError("Q and out are [tokens, heads, D], K and V [tokens, kv_heads, D]")
-    if q_offsets.dim() != 1 or q_offsets.shape != k_offsets.shape or q_offsets.numel() == 0:
+    if len(shape) != 1 or shape != k_offsets.shape or shape[0] == 0:
         raise ValueError("q_offsets and k_offsets have batch + 1 entries")
-    for t in (Q, K, V, out):
-        if t.stride(2) != 1:
-            raise ValueError("the head dimension must be contiguous")
-    if str(Q.dtype) not in ("torch.float16", "torch.bfloat16"):
+    q, k, v, o = Q.stride(), K.stride(), V.stride(), out.stride()
+    if q[2] != 1 or k[2] != 1 or v[2] != 1 or o[2] != 1:
+        raise ValueError("the head dimension must be contiguous")
+    code = _KINDS.get(Q.dtype)
+    if code is None:
         raise ValueError("Q, K and V must be fp16 or bf16")
-    return PackedArgs(Q.shape[2], Q.shape[1], K.shape[1], q_offsets.numel() - 1, Q.shape[0], K.shape[0], int(bool(causal)), _dtype_code(Q), float(scale),
-                      Q.stride(0), Q.stride(1), K.stride(0), K.stride(1), V.stride(0), V.stride(1), out.stride(0), out.stride(1))
+    return PackedArgs(qs[2], qs[1], ks[1], shape[0] - 1, qs[0], ks[0], 1 if causal else 0, code, scale, q[0], q[1], k[0], k[1], v[0], v[1], o[0], o[1])
 
 
 def prefill_packed_workspace(Q, K, V, q_offsets, k_offsets=None, causal: bool = True):
     """Scratch tensor for prefill_packed with tensors of these shapes (it may be empty)."""
-    import torch
     a = _packed_args(Q, K, V, q_offsets, q_offsets if k_offsets is None else k_offsets, causal, 0.0, Q)
-    with _on(Q):
-        return torch.empty(int(lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(a))), dtype=torch.uint8, device=Q.device)
+    return Q.new_empty(_on(_together(Q, (K, V)), lib().b200p_attn_prefill_packed_workspace_bytes, C.byref(a)), dtype=_torch.uint8)
 
 
 def prefill_packed(Q, K, V, q_offsets, k_offsets=None, causal: bool = True, scale: float = 0.0, out=None, workspace=None):
@@ -622,52 +624,51 @@ def prefill_packed(Q, K, V, q_offsets, k_offsets=None, causal: bool = True, scal
     k_offsets[b] .. k_offsets[b + 1] of K and V (int32 CUDA tensors of batch + 1 entries; default: the same rows).  Causal: a sequence's
     last query sees all its keys, each one before it sees one key less, so keys beyond the queries are a cache in front of them.  A
     query without keys gets zeros; rows of out outside all sequences are left as they are.  scale 0: 1 / sqrt(D)."""
-    import torch
     if k_offsets is None:
         k_offsets = q_offsets
     if out is None:
-        out = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
-    _together(Q, (K, V, out), (q_offsets, k_offsets))
+        out = Q.new_empty(Q.shape)
+    device = _together(Q, (K, V, out), (q_offsets, k_offsets))
     a = _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out)
-    with _on(Q):
-        ws, at, n = _scratch(workspace, int(lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(a))), Q)
-        _check(lib().b200p_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), out.data_ptr(),
-                                               C.byref(a), at, n, _stream(Q)), "attn_prefill_packed")
+    L = lib()
+    ws = _scratch(workspace, L.b200p_attn_prefill_packed_workspace_bytes, a, Q, device)
+    _check(_on(device, L.b200p_attn_prefill_packed, Q.data_ptr(), K.data_ptr(), V.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), out.data_ptr(), C.byref(a),
+               None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(Q)), "attn_prefill_packed")
     return out
 
 
 def _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out):
-    if q.dim() != 3 or K_prefix.dim() != 3 or K.dim() != 4 or K_prefix.shape != V_prefix.shape or K.shape != V.shape or out.shape != q.shape:
+    torch = _torch or _bind()
+    qs, ps, ks = q.shape, K_prefix.shape, K.shape
+    if len(qs) != 3 or len(ps) != 3 or len(ks) != 4 or ps != V_prefix.shape or ks != V.shape or out.shape != qs:
         raise ValueError("q and out are [batch, heads, D], the prefix [kv_heads, keys, D], K and V [batch, kv_heads, keys, D]")
-    batch, heads, D = q.shape
-    kv, room, most = K_prefix.shape[0], K_prefix.shape[1], K.shape[2]
-    if K.shape[0] != batch or K.shape[1] != kv or K.shape[3] != D or K_prefix.shape[2] != D:
+    batch, heads, D = qs
+    kv, room, _ = ps
+    most = ks[2]
+    if ks != (batch, kv, most, D) or ps[2] != D:
         raise ValueError("q, the prefix and the caches must agree in batch, key heads and head size")
     n = room if prefix_len is None else int(prefix_len)
     if not 0 <= n <= room:
         raise ValueError(f"prefix_len must be 0 .. {room}")
-    if str(q.dtype) not in ("torch.float16", "torch.bfloat16"):
+    code = _KINDS.get(q.dtype)
+    if code is None:
         raise ValueError("q, K and V must be fp16 or bf16")
-    # a dimension of one element may have any stride
-    own_head, own_batch = K.stride(1) if kv > 1 else most * D, K.stride(0) if batch > 1 else kv * most * D
-    for t in (K_prefix, V_prefix, K, V):
-        if t.stride(-1) != 1 or (t.shape[-2] > 1 and t.stride(-2) != D):
-            raise ValueError("the rows of a key head must follow one another")
-    if K_prefix.stride() != V_prefix.stride() or K.stride() != V.stride():
+    sq, so, sp, sk = q.stride(), out.stride(), K_prefix.stride(), K.stride()
+    if sp != V_prefix.stride() or sk != V.stride():
         raise ValueError("K and V must have the same strides")
-    for t in (q, out):
-        if t.stride(2) != 1 or (heads > 1 and t.stride(1) != D):
-            raise ValueError("the heads of q and of out must follow one another")
-    return SharedArgs(D, heads, kv, batch, n, most, _dtype_code(q), float(scale), K_prefix.stride(0) if kv > 1 else room * D, own_head, own_batch,
-                      q.stride(0) if batch > 1 else heads * D, out.stride(0) if batch > 1 else heads * D)
+    # a dimension of one element may have any stride
+    if sp[2] != 1 or sk[3] != 1 or (room > 1 and sp[1] != D) or (most > 1 and sk[2] != D):
+        raise ValueError("the rows of a key head must follow one another")
+    if sq[2] != 1 or so[2] != 1 or (heads > 1 and (sq[1] != D or so[1] != D)):
+        raise ValueError("the heads of q and of out must follow one another")
+    return SharedArgs(D, heads, kv, batch, n, most, code, scale, sp[0] if kv > 1 else room * D, sk[1] if kv > 1 else most * D,
+                      sk[0] if batch > 1 else kv * (sk[1] if kv > 1 else most * D), sq[0] if batch > 1 else heads * D, so[0] if batch > 1 else heads * D)
 
 
 def decode_shared_workspace(q, K_prefix, K, prefix_len=None):
     """Scratch tensor for decode_shared with tensors of these shapes (it may be empty)."""
-    import torch
     a = _shared_args(q, K_prefix, K_prefix, K, K, prefix_len, 0.0, q)
-    with _on(q):
-        return torch.empty(int(lib().b200p_attn_decode_shared_workspace_bytes(C.byref(a))), dtype=torch.uint8, device=q.device)
+    return q.new_empty(_on(_together(q, (K_prefix, K)), lib().b200p_attn_decode_shared_workspace_bytes, C.byref(a)), dtype=_torch.uint8)
 
 
 def decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len=None, scale: float = 0.0, out=None, workspace=None):
@@ -675,17 +676,16 @@ def decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len=None, scale: 
     attends to the first prefix_len keys of K_prefix / V_prefix [kv_heads, max_prefix, D] (default: all) and to the first lengths[b]
     keys of its own cache K / V [batch, kv_heads, max_own, D].  lengths: int32 CUDA tensor, read on the device.  A sequence without
     keys gets zeros.  scale 0: 1 / sqrt(D)."""
-    import torch
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _together(q, (K_prefix, V_prefix, K, V, out), (lengths,))
+        out = q.new_empty(q.shape)
+    device = _together(q, (K_prefix, V_prefix, K, V, out), (lengths,))
     a = _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out)
-    if lengths.dim() != 1 or lengths.numel() != q.shape[0]:
+    if lengths.shape != q.shape[:1]:
         raise ValueError("lengths has one entry per sequence")
-    with _on(q):
-        ws, at, n = _scratch(workspace, int(lib().b200p_attn_decode_shared_workspace_bytes(C.byref(a))), q)
-        _check(lib().b200p_attn_decode_shared(q.data_ptr(), K_prefix.data_ptr(), V_prefix.data_ptr(), K.data_ptr(), V.data_ptr(), lengths.data_ptr(),
-                                              out.data_ptr(), C.byref(a), at, n, _stream(q)), "attn_decode_shared")
+    L = lib()
+    ws = _scratch(workspace, L.b200p_attn_decode_shared_workspace_bytes, a, q, device)
+    _check(_on(device, L.b200p_attn_decode_shared, q.data_ptr(), K_prefix.data_ptr(), V_prefix.data_ptr(), K.data_ptr(), V.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+               C.byref(a), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(q)), "attn_decode_shared")
     return out
 
 
@@ -697,22 +697,21 @@ def adjust_logits(logits, prompt=None, prompt_lengths=None, tokens=None, token_l
     (ids int32, values fp32, both [rows, n]); then tokens whose bit in `mask` (int32 [masks, (vocab + 31) // 32]) is 0 become -inf, where
     mask_rows (int32 [rows], default: row i takes mask i) names a row's mask or, with -1, none.  Ids outside the vocabulary are
     ignored.  out may be logits itself."""
-    import torch
+    torch = _torch or _bind()
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)
     if logits.dim() != 2 or out.shape != logits.shape:
         raise ValueError("logits and out are [rows, vocab]")
     R, V = logits.shape
-    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(logits.dtype)
+    code = F32 if logits.dtype == torch.float32 else _KINDS.get(logits.dtype)
     if code is None:
         raise ValueError("logits must be fp32, fp16 or bf16")
-    words = (V + 31) // 32
-    _together(logits, (out,), [t for t in (prompt, prompt_lengths, tokens, token_lengths, bias_ids, mask, mask_rows) if t is not None])
+    device = _together(logits, (out,), [t for t in (prompt, prompt_lengths, tokens, token_lengths, bias_ids, mask, mask_rows) if t is not None])
     for t in (repetition, presence, frequency, bias_values):
-        if t is not None and (t.get_device() != logits.get_device() or t.dtype != torch.float32 or not t.is_contiguous()):
+        if t is not None and (t.get_device() != device or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError("penalties and bias values must be contiguous fp32 tensors on the logits' device")
     for t in (prompt_lengths, token_lengths, repetition, presence, frequency, mask_rows):
-        if t is not None and tuple(t.shape) != (R,):
+        if t is not None and t.shape != (R,):
             raise ValueError("lengths, penalties and mask_rows have one entry per row")
     for t in (prompt, tokens, bias_ids):
         if t is not None and (t.dim() != 2 or t.shape[0] != R):
@@ -721,20 +720,23 @@ def adjust_logits(logits, prompt=None, prompt_lengths=None, tokens=None, token_l
         raise ValueError("bias_ids and bias_values go together")
     if (prompt is None and prompt_lengths is not None) or (tokens is None and token_lengths is not None) or (mask is None and mask_rows is not None):
         raise ValueError("lengths need their ids, mask_rows needs a mask")
-    if mask is not None and (mask.dim() != 2 or mask.shape[1] != words or (mask_rows is None and mask.shape[0] != R)):
-        raise ValueError(f"mask is [masks, {words}], with one mask per row or mask_rows")
-    for t in (logits, out):
-        if (V > 1 and t.stride(1) != 1) or (R > 1 and t.stride(0) < V):
-            raise ValueError("the logits of a row must follow one another")
+    if mask is not None and (mask.dim() != 2 or mask.shape[1] != (V + 31) // 32 or (mask_rows is None and mask.shape[0] != R)):
+        raise ValueError(f"mask is [masks, {(V + 31) // 32}], with one mask per row or mask_rows")
+    si, so = logits.stride(), out.stride()
+    if (V > 1 and (si[1] != 1 or so[1] != 1)) or (R > 1 and (si[0] < V or so[0] < V)):
+        raise ValueError("the logits of a row must follow one another")
     if R == 0 or V == 0:
         return out
-    ptr = lambda t: t.data_ptr() if t is not None and t.numel() else None
-    width = lambda t: t.shape[1] if t is not None else 0
-    a = LogitsArgs(code, R, V, width(prompt), width(tokens), width(bias_ids), mask.shape[0] if mask is not None else 0,
-                   logits.stride(0) if R > 1 else V, out.stride(0) if R > 1 else V, ptr(prompt), ptr(prompt_lengths), ptr(tokens), ptr(token_lengths),
-                   ptr(repetition), ptr(presence), ptr(frequency), ptr(bias_ids), ptr(bias_values), ptr(mask), ptr(mask_rows))
-    with _on(logits):
-        _check(lib().b200p_logits_adjust(logits.data_ptr(), out.data_ptr(), C.byref(a), _stream(logits)), "logits_adjust")
+
+    def ptr(t):
+        return None if t is None else t.data_ptr() or None        # an empty tensor has no address
+
+    def width(t):
+        return 0 if t is None else t.shape[1]
+    a = LogitsArgs(code, R, V, width(prompt), width(tokens), width(bias_ids), 0 if mask is None else mask.shape[0], si[0] if R > 1 else V, so[0] if R > 1 else V,
+                   ptr(prompt), ptr(prompt_lengths), ptr(tokens), ptr(token_lengths), ptr(repetition), ptr(presence), ptr(frequency), ptr(bias_ids), ptr(bias_values),
+                   ptr(mask), ptr(mask_rows))
+    _check(_on(device, lib().b200p_logits_adjust, logits.data_ptr(), out.data_ptr(), C.byref(a), _stream(logits)), "logits_adjust")
     return out
 
 

@@ -21,6 +21,7 @@ constexpr int kOwnWarps = 4;
 constexpr int kOwnThreads = kOwnWarps * 32;
 constexpr int kKeyBlock = 16;                    // keys of a warp's step
 constexpr int kMostOwnCluster = 8;
+constexpr int kMostSplits = 160;                 // of the prefix: one for each SM, for a single key head
 
 struct OwnParams {
     const void *q, *Kp, *Vp, *K, *V;
@@ -39,11 +40,6 @@ __device__ __forceinline__ uint32_t transposed_8x8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint4 load16(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ float load_cluster_f32(uint32_t smem, uint32_t cta) {
     uint32_t a;
     float v;
@@ -51,163 +47,309 @@ __device__ __forceinline__ float load_cluster_f32(uint32_t smem, uint32_t cta) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 load_cluster_f32x4(uint32_t smem, uint32_t cta) {
+    uint32_t a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(cta));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
 __device__ __forceinline__ float weight_of(float m, float most) { return exp2f(m - (most == -INFINITY ? 0.f : most)); }
 
-// One cluster of `gridDim.x` CTAs per (sequence, key head, 8 * NT query rows); a warp takes every (warps of the cluster)-th block of
-// 16 keys.  A step is S^T = K Q^T and O^T += V^T P^T with mma.sync m16n8k16 (keys, then head columns, in the 16 rows; the query
-// heads of a group in the 8 columns, so that 8 heads fill an instruction).  Operands come straight from global memory, 16 bytes per
-// lane and load: the contraction runs over the head columns in the order in which the lanes hold them, for K and Q alike; V's rows
-// are paired up by byte permutes.  No shared memory or barrier stands between the loads and the products, a warp has 8 KB (heads of
-// 128) in flight, 16 warps fit an SM.  Rows past the length are not read: their registers are zero.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kOwnThreads, NT == 1 ? 4 : D == 64 ? 3 : 2)
-own_kernel(const OwnParams p) {
-    constexpr int KC = D / 32, VC = D / 64, R = 8 * NT;
-    __shared__ __align__(16) float s_o[kOwnWarps][R][D + 4];
-    __shared__ float s_ml[kOwnWarps][R][2];
-    __shared__ __align__(16) float s_sum[R][D];           // the CTA's result, for the cluster
-    __shared__ float s_sum_ml[R][2];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
-    const int ctas = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y / p.row_groups, r0 = (blockIdx.y % p.row_groups) * R, b = blockIdx.z;
-    const int own = p.max_own > 0 ? min(max(p.lengths[b], 0), p.max_own) : 0;
-    const int rows = min(R, p.group - r0), nQH = p.nKVH * p.group, head0 = kvh * p.group + r0;
+// Up to 8 * NT query rows against blocks of 16 keys by one warp.  A step is S^T = K Q^T and O^T += V^T P^T with mma.sync m16n8k16: keys,
+// then head columns, in the 16 rows, the query rows in the 8 columns, so that 8 of them fill an instruction.  Operands come straight
+// from global memory, 16 bytes per lane and load: the contraction runs over the head columns in the order in which the lanes hold
+// them, for K and Q alike; V's rows are paired up by byte permutes.  No shared memory and no barrier stands between the loads and the
+// products; a warp has 8 KB (heads of 128) in flight.  Rows past the run's end are not read: their registers are zero.
+// Lane (g, t4) = (lane / 4, lane % 4).
+template <typename T, int D, int NT, bool CACHED> struct KeyWalk {
+    static constexpr int KC = D / 32, VC = D / 64, R = 8 * NT;
+    uint4 qf[NT][KC];                                     // row n * 8 + g, columns 32 c + 8 t4 ..
+    uint4 kf[2][KC], vf[4][VC];                           // keys g, g + 8, the same columns; keys 2 t4, + 1, + 8, + 9, columns 64 c + 8 g ..
+    float o[NT][D / 16][4];                               // tile (c, i): columns d = 64 c + 8 g + 2 i and + 1 of rows n * 8 + 2 t4 and + 1
+    float m[NT][2], l[NT][2];                             // of those rows; l: over this lane's keys
+    int g, t4;
 
-    // Q: column n of the B operand is query row r0 + n; lane (g, t4) has row g's columns 32 c + 8 t4 ..
-    uint4 qf[NT][KC];
-    #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const T* row = static_cast<const T*>(p.q) + b * p.q_batch + (long long)(head0 + n * 8 + g) * D + t4 * 8;
+    __device__ __forceinline__ KeyWalk() : g(threadIdx.x % 32 / 4), t4(threadIdx.x % 4) {
         #pragma unroll
-        for (int c = 0; c < KC; ++c) qf[n][c] = n * 8 + g < rows ? *reinterpret_cast<const uint4*>(row + 32 * c) : make_uint4(0, 0, 0, 0);
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY; l[n][0] = l[n][1] = 0.f;
+            #pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+        }
     }
-    float o[NT][D / 16][4] = {};                          // tile (c, i): rows d = 64 c + 8 g + 2 i and + 1, columns 2 t4 and + 1
-    float m[NT][2], l[NT][2];
-    #pragma unroll
-    for (int n = 0; n < NT; ++n) { m[n][0] = m[n][1] = -INFINITY; l[n][0] = l[n][1] = 0.f; }
-
-    const int prefix_blocks = (p.prefix_here + kKeyBlock - 1) / kKeyBlock, blocks = prefix_blocks + (own + kKeyBlock - 1) / kKeyBlock;
-    const long long own_at = b * p.own_batch + kvh * p.own_head, prefix_at = kvh * p.prefix_head;
-    for (int j = rank * kOwnWarps + warp; j < blocks; j += ctas * kOwnWarps) {
-        const bool shared = j < prefix_blocks;
-        const int key0 = (shared ? j : j - prefix_blocks) * kKeyBlock, there = (shared ? p.prefix_here : own) - key0;      // keys of the block
-        const long long at = (shared ? prefix_at : own_at) + (long long)key0 * D;
-        const T* K = static_cast<const T*>(shared ? p.Kp : p.K) + at;
-        const T* V = static_cast<const T*>(shared ? p.Vp : p.V) + at;
-        uint4 kf[2][KC], vf[4][VC];
+    static __device__ __forceinline__ uint4 load16(const T* p) {
+        uint4 v;
+        if constexpr (CACHED) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        else asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        return v;
+    }
+    // row: this lane's row (n * 8 + g) or null
+    __device__ __forceinline__ void load_q(int n, const T* row) {
+        #pragma unroll
+        for (int c = 0; c < KC; ++c) qf[n][c] = row ? *reinterpret_cast<const uint4*>(row + 32 * c + 8 * t4) : make_uint4(0, 0, 0, 0);
+    }
+    // the block's first row, and how many rows there are
+    __device__ __forceinline__ void load_k(const T* K, int there) {
         #pragma unroll
         for (int h = 0; h < 2; ++h)
             #pragma unroll
             for (int c = 0; c < KC; ++c) kf[h][c] = g + 8 * h < there ? load16(K + (g + 8 * h) * D + 32 * c + 8 * t4) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load_v(const T* V, int there) {
         #pragma unroll
         for (int h = 0; h < 4; ++h) {
             const int key = 2 * t4 + (h & 1) + 8 * (h >> 1);
             #pragma unroll
             for (int c = 0; c < VC; ++c) vf[h][c] = key < there ? load16(V + key * D + 64 * c + 8 * g) : make_uint4(0, 0, 0, 0);
         }
+    }
+    // values that were loaded ahead of knowing the end
+    __device__ __forceinline__ void drop_v(int there) {
+        #pragma unroll
+        for (int h = 0; h < 4; ++h)
+            #pragma unroll
+            for (int c = 0; c < VC; ++c) if (2 * t4 + (h & 1) + 8 * (h >> 1) >= there) vf[h][c] = make_uint4(0, 0, 0, 0);
+    }
+    // The block that is loaded.  next_k(): called as soon as K's registers are free.
+    template <typename F> __device__ __forceinline__ void step(int there, float scale_log2, F&& next_k) {
+        float s[NT][4];                                   // keys g and g + 8, rows 2 t4 and + 1
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};            // keys g and g + 8, rows 2 t4 and + 1
+            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
             #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 const uint32_t a0[4] = {kf[0][c].x, kf[1][c].x, kf[0][c].y, kf[1][c].y}, a1[4] = {kf[0][c].z, kf[1][c].z, kf[0][c].w, kf[1][c].w};
-                mma_16816<T>(s, a0, qf[n][c].x, qf[n][c].y);
-                mma_16816<T>(s, a1, qf[n][c].z, qf[n][c].w);
+                mma_16816<T>(s[n], a0, qf[n][c].x, qf[n][c].y);
+                mma_16816<T>(s[n], a1, qf[n][c].z, qf[n][c].w);
             }
-            if (g >= there) s[0] = s[1] = -INFINITY;
-            if (g + 8 >= there) s[2] = s[3] = -INFINITY;
+        }
+        next_k();
+        uint32_t pt[NT][2];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (g >= there) s[n][0] = s[n][1] = -INFINITY;
+            if (g + 8 >= there) s[n][2] = s[n][3] = -INFINITY;
             float alpha[2];
             #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float x = fmaxf(s[e], s[2 + e]);
+                float x = fmaxf(s[n][e], s[n][2 + e]);
                 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                const float next = fmaxf(m[n][e], x * p.scale_log2), ref = next == -INFINITY ? 0.f : next;
+                const float most = fmaxf(m[n][e], x * scale_log2), ref = most == -INFINITY ? 0.f : most;      // nothing but -inf so far: weights of 0
                 alpha[e] = fast_exp2(m[n][e] - ref);
-                m[n][e] = next;
-                s[e] = fast_exp2(fmaf(s[e], p.scale_log2, -ref));
-                s[2 + e] = fast_exp2(fmaf(s[2 + e], p.scale_log2, -ref));
-                l[n][e] = l[n][e] * alpha[e] + (s[e] + s[2 + e]);
+                m[n][e] = most;
+                s[n][e] = fast_exp2(fmaf(s[n][e], scale_log2, -ref));
+                s[n][2 + e] = fast_exp2(fmaf(s[n][2 + e], scale_log2, -ref));
+                l[n][e] = l[n][e] * alpha[e] + (s[n][e] + s[n][2 + e]);
             }
             if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
                 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) { o[n][i][0] *= alpha[0]; o[n][i][1] *= alpha[1]; o[n][i][2] *= alpha[0]; o[n][i][3] *= alpha[1]; }
             }
-            const uint32_t b0 = transposed_8x8(pack2<T>(s[0], s[1])), b1 = transposed_8x8(pack2<T>(s[2], s[3]));
+            pt[n][0] = transposed_8x8(pack2<T>(s[n][0], s[n][1])); pt[n][1] = transposed_8x8(pack2<T>(s[n][2], s[n][3]));
+        }
+        #pragma unroll
+        for (int c = 0; c < VC; ++c) {
+            const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vf[0][c]); const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vf[1][c]);
+            const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vf[2][c]); const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vf[3][c]);
             #pragma unroll
-            for (int c = 0; c < VC; ++c) {
-                const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vf[0][c]); const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vf[1][c]);
-                const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vf[2][c]); const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vf[3][c]);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a[4] = {__byte_perm(v0[i], v1[i], 0x5410), __byte_perm(v0[i], v1[i], 0x7632), __byte_perm(v2[i], v3[i], 0x5410), __byte_perm(v2[i], v3[i], 0x7632)};
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t a[4] = {__byte_perm(v0[i], v1[i], 0x5410), __byte_perm(v0[i], v1[i], 0x7632), __byte_perm(v2[i], v3[i], 0x5410), __byte_perm(v2[i], v3[i], 0x7632)};
-                    mma_16816<T>(o[n][c * 4 + i], a, b0, b1);
-                }
+                for (int n = 0; n < NT; ++n) mma_16816<T>(o[n][c * 4 + i], a, pt[n][0], pt[n][1]);
             }
         }
     }
-    // the warp's result
+    // Row n * 8 + 2 t4 + e: put(row, maximum, sum over all lanes) by the lanes with g = 0, then every lane's columns, four at a time.
+    template <typename ML, typename O4> __device__ __forceinline__ void result(ML&& put_ml, O4&& put_o) {
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = l[n][e];
+                #pragma unroll
+                for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+                const int row = n * 8 + 2 * t4 + e;
+                if (g == 0) put_ml(row, m[n][e], x);
+                #pragma unroll
+                for (int c = 0; c < VC; ++c)
+                    #pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        put_o(row, 64 * c + 8 * g + 4 * h, make_float4(o[n][c * 4 + 2 * h][e], o[n][c * 4 + 2 * h][2 + e], o[n][c * 4 + 2 * h + 1][e], o[n][c * 4 + 2 * h + 1][2 + e]));
+            }
+    }
+};
+
+// The prefix for batches whose rows are few (plan_shared): warps of a CTA that share the keys of its split have other query rows
+// (K and V then come from L1 for all but the first of them), WK of them take every WK-th block of 16 keys for the same rows and
+// meet in shared memory.  Small CTAs, so that the next launch's find room beside them and read the sequences' own keys meanwhile.
+struct PrefixParams {
+    const void *q, *K, *V;
+    int rows, group, nKVH, keys, keys_per_split, row_groups;     // rows: batch * group, of a key head; row_groups: CTAs over them
+    long long head, q_batch;
+    float scale_log2;
+    float *part_o, *part_ml;
+};
+template <typename T, int D, int NT, int WK>
+__global__ void __launch_bounds__(kOwnThreads, NT == 1 ? 4 : D == 64 ? 3 : 2)
+prefix_kernel(const PrefixParams p) {
+    constexpr int WR = kOwnWarps / WK, R = 8 * NT;
+    __shared__ __align__(16) float s_o[WK > 1 ? kOwnWarps : 1][R][D + 4];
+    __shared__ float s_ml[kOwnWarps][R][2];
+    griddep_launch_dependents();
+    const int warp = threadIdx.x / 32, split = blockIdx.x, kvh = blockIdx.y / p.row_groups, rg = blockIdx.y % p.row_groups;
+    const int row0 = (rg * WR + warp / WK) * R, nQH = p.nKVH * p.group;
+    KeyWalk<T, D, NT, true> w;
+    #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int row = row0 + n * 8 + w.g, b = row / p.group;
+        w.load_q(n, row < p.rows ? static_cast<const T*>(p.q) + b * p.q_batch + (long long)(kvh * p.group + row - b * p.group) * D : nullptr);
+    }
+    const int k0 = split * p.keys_per_split, keys = min(p.keys_per_split, p.keys - k0), blocks = (keys + kKeyBlock - 1) / kKeyBlock;
+    const T* const K = static_cast<const T*>(p.K) + kvh * p.head + (long long)k0 * D; const T* const V = static_cast<const T*>(p.V) + kvh * p.head + (long long)k0 * D;
+    if (row0 < p.rows) {
+        int j = warp % WK;
+        if (j < blocks) { w.load_k(K + j * kKeyBlock * D, keys - j * kKeyBlock); w.load_v(V + j * kKeyBlock * D, keys - j * kKeyBlock); }
+        for (; j < blocks; j += WK) {
+            const int next = (j + WK) * kKeyBlock;
+            w.step(keys - j * kKeyBlock, p.scale_log2, [&] { if (next < keys) w.load_k(K + (long long)next * D, keys - next); });
+            if (next < keys) w.load_v(V + (long long)next * D, keys - next);
+        }
+    }
+    // row r of the partial results: [split][sequence][head]
+    auto part_row = [&](int row) { const int b = row / p.group; return (size_t(split) * (p.rows / p.group) + b) * nQH + kvh * p.group + row - b * p.group; };
+    if constexpr (WK == 1) {
+        w.result([&](int row, float m, float l) { if (row0 + row < p.rows) *reinterpret_cast<float2*>(&p.part_ml[2 * part_row(row0 + row)]) = make_float2(m, l); },
+                 [&](int row, int d, float4 v) { if (row0 + row < p.rows) *reinterpret_cast<float4*>(&p.part_o[part_row(row0 + row) * D + d]) = v; });
+    } else {
+        w.result([&](int row, float m, float l) { s_ml[warp][row][0] = m; s_ml[warp][row][1] = l; }, [&](int row, int d, float4 v) { *reinterpret_cast<float4*>(&s_o[warp][row][d]) = v; });
+        __syncthreads();
+        for (int i = threadIdx.x; i < WR * R * (D / 4); i += kOwnThreads) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4, w0 = r / R * WK, in = r % R, row = rg * WR * R + r;
+            if (row >= p.rows) break;
+            float most = -INFINITY, sum = 0.f;
+            #pragma unroll
+            for (int k = 0; k < WK; ++k) most = fmaxf(most, s_ml[w0 + k][in][0]);
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            #pragma unroll
+            for (int k = 0; k < WK; ++k) {
+                const float f = weight_of(s_ml[w0 + k][in][0], most);
+                const float4 v = *reinterpret_cast<const float4*>(&s_o[w0 + k][in][d]);
+                sum += f * s_ml[w0 + k][in][1];
+                x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
+            }
+            const size_t at = part_row(row);
+            *reinterpret_cast<float4*>(&p.part_o[at * D + d]) = x;
+            if (d == 0) *reinterpret_cast<float2*>(&p.part_ml[2 * at]) = make_float2(most, sum);
+        }
+    }
+}
+
+// The sequences' own keys (and the prefix's where it has no launch of its own), and the merge.  One cluster of `gridDim.x` CTAs per
+// (sequence, key head, 8 * NT query rows); a warp takes every (warps of the cluster)-th block of 16 keys.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kOwnThreads, NT == 1 ? 4 : D == 64 ? 3 : 2)
+own_kernel(const OwnParams p) {
+    constexpr int R = 8 * NT;
+    __shared__ __align__(16) float s_o[kOwnWarps][R][D + 4];
+    __shared__ float s_ml[kOwnWarps][R][2];
+    __shared__ float s_sum_ml[R][2];                      // the CTA's, for the cluster; its O takes the first warp's place
+    __shared__ float s_w[R][kMostOwnCluster + kMostSplits];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int ctas = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y / p.row_groups, r0 = (blockIdx.y % p.row_groups) * R, b = blockIdx.z;
+    const int rows = min(R, p.group - r0), nQH = p.nKVH * p.group, head0 = kvh * p.group + r0;
+
+    KeyWalk<T, D, NT, false> w;
+    const int prefix_blocks = (p.prefix_here + kKeyBlock - 1) / kKeyBlock, stride = ctas * kOwnWarps;
+    const T* const own_k = static_cast<const T*>(p.K) + b * p.own_batch + kvh * p.own_head; const T* const own_v = static_cast<const T*>(p.V) + b * p.own_batch + kvh * p.own_head;
+    const T* const prefix_k = static_cast<const T*>(p.Kp) + kvh * p.prefix_head; const T* const prefix_v = static_cast<const T*>(p.Vp) + kvh * p.prefix_head;
+    auto first_key = [&](int j) { return (j < prefix_blocks ? j : j - prefix_blocks) * kKeyBlock; };
+    auto keys_of = [&](int j, int own) { return (j < prefix_blocks ? p.prefix_here : own) - first_key(j); };
+    auto load_k = [&](int j, int own) { w.load_k((j < prefix_blocks ? prefix_k : own_k) + (long long)first_key(j) * D, keys_of(j, own)); };
+    auto load_v = [&](int j, int own) { w.load_v((j < prefix_blocks ? prefix_v : own_v) + (long long)first_key(j) * D, keys_of(j, own)); };
+    // the first block does not wait for the length: up to the cache's end the rows are there, whatever they hold
+    int j = rank * kOwnWarps + warp;
+    load_k(j, p.max_own);
+    load_v(j, p.max_own);
     #pragma unroll
     for (int n = 0; n < NT; ++n)
-        #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float x = l[n][e];
-            #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-            const int row = n * 8 + 2 * t4 + e;
-            if (g == 0) { s_ml[warp][row][0] = m[n][e]; s_ml[warp][row][1] = x; }
-            #pragma unroll
-            for (int c = 0; c < VC; ++c)
-                #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    *reinterpret_cast<float4*>(&s_o[warp][row][64 * c + 8 * g + 4 * h]) =
-                        make_float4(o[n][c * 4 + 2 * h][e], o[n][c * 4 + 2 * h][2 + e], o[n][c * 4 + 2 * h + 1][e], o[n][c * 4 + 2 * h + 1][2 + e]);
-        }
+        w.load_q(n, n * 8 + w.g < rows ? static_cast<const T*>(p.q) + b * p.q_batch + (long long)(head0 + n * 8 + w.g) * D : nullptr);
+    const int own = p.max_own > 0 ? min(max(p.lengths[b], 0), p.max_own) : 0;
+    const int blocks = prefix_blocks + (own + kKeyBlock - 1) / kKeyBlock;
+    if (j < blocks) w.drop_v(keys_of(j, own));
+    for (; j < blocks; j += stride) {
+        w.step(keys_of(j, own), p.scale_log2, [&] { if (j + stride < blocks) load_k(j + stride, own); });
+        if (j + stride < blocks) load_v(j + stride, own);
+    }
+    w.result([&](int row, float m, float l) { s_ml[warp][row][0] = m; s_ml[warp][row][1] = l; }, [&](int row, int d, float4 v) { *reinterpret_cast<float4*>(&s_o[warp][row][d]) = v; });
     __syncthreads();
     // the CTA's, where a cluster follows
     if (ctas > 1) {
         for (int i = threadIdx.x; i < rows * D; i += kOwnThreads) {
             const int row = i / D, d = i % D;
             float most = -INFINITY, sum = 0.f, x = 0.f;
-            for (int w = 0; w < kOwnWarps; ++w) most = fmaxf(most, s_ml[w][row][0]);
-            for (int w = 0; w < kOwnWarps; ++w) { const float f = weight_of(s_ml[w][row][0], most); sum += f * s_ml[w][row][1]; x += f * s_o[w][row][d]; }
-            s_sum[row][d] = x;
+            for (int k = 0; k < kOwnWarps; ++k) most = fmaxf(most, s_ml[k][row][0]);
+            for (int k = 0; k < kOwnWarps; ++k) { const float f = weight_of(s_ml[k][row][0], most); sum += f * s_ml[k][row][1]; x += f * s_o[k][row][d]; }
+            s_o[0][row][d] = x;
             if (d == 0) { s_sum_ml[row][0] = most; s_sum_ml[row][1] = sum; }
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     griddep_wait();                                       // the prefix's splits are there
-    const int share = (rows * D + ctas - 1) / ctas, last = min(rows * D, (rank + 1) * share);
+    // every part's weight in the sum, 2^(m_i - m) / l, a warp per row: the warps (or the cluster's CTAs), then the prefix's splits
+    const int parts = ctas > 1 ? ctas : kOwnWarps;
+    const size_t part0 = size_t(b) * nQH + head0, next = size_t(p.batch) * nQH;
+    for (int row = warp; row < rows; row += kOwnWarps) {
+        float2 ml[kMostSplits / 32 + 1];                  // lane i: part i, then the splits i, 32 + i, ...
+        ml[0] = make_float2(-INFINITY, 0.f);
+        if (lane < parts)
+            ml[0] = ctas > 1 ? make_float2(load_cluster_f32(dme::smem_addr(&s_sum_ml[row][0]), lane), load_cluster_f32(dme::smem_addr(&s_sum_ml[row][1]), lane))
+                             : make_float2(s_ml[lane][row][0], s_ml[lane][row][1]);
+        float most = ml[0].x;
+        #pragma unroll
+        for (int k = 0; k < kMostSplits / 32; ++k) {
+            const int s = 32 * k + lane;
+            ml[k + 1] = s < p.splits ? *reinterpret_cast<const float2*>(&p.part_ml[2 * (part0 + row + s * next)]) : make_float2(-INFINITY, 0.f);
+            most = fmaxf(most, ml[k + 1].x);
+        }
+        #pragma unroll
+        for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        float sum = 0.f;
+        #pragma unroll
+        for (int k = 0; k <= kMostSplits / 32; ++k) {
+            const float f = ml[k].y == 0.f ? 0.f : weight_of(ml[k].x, most);        // a sum of 0: no key
+            sum += f * ml[k].y;
+            ml[k].x = f;
+        }
+        #pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float inv = p.prefix_len + own > 0 ? 1.f / sum : 0.f;
+        if (lane < parts) s_w[row][lane] = ml[0].x * inv;
+        #pragma unroll
+        for (int k = 0; k < kMostSplits / 32; ++k) if (32 * k + lane < p.splits) s_w[row][kMostOwnCluster + 32 * k + lane] = ml[k + 1].x * inv;
+    }
+    __syncthreads();
+    // four columns per thread
+    const int quads = rows * (D / 4), share = (quads + ctas - 1) / ctas, last = min(quads, (rank + 1) * share);
     for (int i = rank * share + threadIdx.x; i < last; i += kOwnThreads) {
-        const int row = i / D, d = i % D;
-        const size_t part = size_t(b) * nQH + head0 + row, next = size_t(p.batch) * nQH;
-        float most = -INFINITY;
-        float om[kMostOwnCluster], ol[kMostOwnCluster], ox[kMostOwnCluster];
-        const int parts = ctas > 1 ? ctas : kOwnWarps;
-        #pragma unroll
-        for (int w = 0; w < kMostOwnCluster; ++w) {
-            if (w >= parts) break;
-            if (ctas > 1) {
-                om[w] = load_cluster_f32(dme::smem_addr(&s_sum_ml[row][0]), w); ol[w] = load_cluster_f32(dme::smem_addr(&s_sum_ml[row][1]), w);
-                ox[w] = load_cluster_f32(dme::smem_addr(&s_sum[row][d]), w);
-            } else { om[w] = s_ml[w][row][0]; ol[w] = s_ml[w][row][1]; ox[w] = s_o[w][row][d]; }
-            most = fmaxf(most, om[w]);
-        }
-        for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.part_ml[2 * (part + s * next)]);
-        float sum = 0.f, x = 0.f;
-        #pragma unroll
-        for (int w = 0; w < kMostOwnCluster; ++w) {
-            if (w >= parts) break;
-            const float f = weight_of(om[w], most);
-            sum += f * ol[w]; x += f * ox[w];
-        }
+        const int row = i / (D / 4), d = i % (D / 4) * 4;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        auto add = [&](float f, const float4& v) { x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w; };
+        const float* o_part = p.part_o + (part0 + row) * D + d;
+        #pragma unroll 8
         for (int s = 0; s < p.splits; ++s) {
-            const float2 ml = *reinterpret_cast<const float2*>(&p.part_ml[2 * (part + s * next)]);
-            if (ml.y == 0.f) continue;                    // no key: nothing was stored
-            const float f = weight_of(ml.x, most);
-            sum += f * ml.y; x += f * p.part_o[(part + s * next) * D + d];
+            const float f = s_w[row][kMostOwnCluster + s];
+            const float4 v = *reinterpret_cast<const float4*>(o_part + s * next * D);
+            if (f != 0.f) add(f, v);                      // where a split had no key for the row nothing was stored
         }
-        static_cast<T*>(p.o)[b * p.o_batch + (long long)(head0 + row) * D + d] = from_float<T>(p.prefix_len + own > 0 ? x / sum : 0.f);
+        for (int k = 0; k < parts; ++k) {
+            const float4 v = ctas > 1 ? load_cluster_f32x4(dme::smem_addr(&s_o[0][row][d]), k) : *reinterpret_cast<const float4*>(&s_o[k][row][d]);
+            add(s_w[row][k], v);
+        }
+        T* y = static_cast<T*>(p.o) + b * p.o_batch + (long long)(head0 + row) * D + d;
+        *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
     }
     if (ctas > 1) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");       // nobody leaves while a peer reads here
@@ -216,23 +358,44 @@ own_kernel(const OwnParams p) {
 }
 
 // How a call is run.
+enum PrefixKind { PREFIX_NONE, PREFIX_HERE, PREFIX_WARPS, PREFIX_TILES };       // no keys; by own_kernel; prefix_kernel; the tcgen05 kernel
 struct SharedPlan {
-    bool prefix_apart;           // the prefix in a launch of its own
-    int splits, span;            // of that launch
-    int cluster, rows;           // CTAs and query rows (8 or 16) of a unit of the second
+    int prefix;
+    int splits, span;            // of the prefix's launch; span: tiles of an item (PREFIX_TILES)
+    int keys_per_split, wk, nt;  // PREFIX_WARPS
+    int cluster, rows;           // CTAs and query rows (8 or 16) of a unit of the second launch
     size_t off_ml, ws_bytes;
 };
 
 SharedPlan plan_shared(const b200p_shared_args& a) {
     SharedPlan pl{};
     const int sms = sm_count() > 0 ? sm_count() : 148, group = a.nQHeads / a.nKVHeads;
+    const long long rows = (long long)a.batch * group, blocks = (a.prefix_len + kKeyBlock - 1) / kKeyBlock;
     pl.rows = group <= 8 ? 8 : 16;
     const long long units = (long long)a.batch * a.nKVHeads * ((group + pl.rows - 1) / pl.rows);
-    pl.prefix_apart = a.prefix_len > 0 && (long long)a.batch * a.prefix_len > 4096;
-    if (pl.prefix_apart) {
+    if (a.prefix_len == 0) pl.prefix = PREFIX_NONE;
+    else if ((long long)a.batch * a.prefix_len <= 4096) pl.prefix = PREFIX_HERE;
+    else pl.prefix = rows * a.prefix_len * a.nKVHeads * a.D <= (1LL << 32) ? PREFIX_WARPS : PREFIX_TILES;
+    const int forced = tuning(KNOB_SHARED_PREFIX, 0);
+    if (a.prefix_len > 0 && forced >= PREFIX_HERE && forced <= PREFIX_TILES) pl.prefix = forced;
+    if (pl.prefix == PREFIX_WARPS) {
+        pl.nt = rows <= 8 ? 1 : 2;
+        const long long warps = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
+        const int wr = warps >= 3 ? 4 : int(warps);
+        pl.wk = kOwnWarps / wr;
+        const long long base = a.nKVHeads * ((warps + wr - 1) / wr), least = 2 * pl.wk;        // blocks of a split
+        long long s = tuning(KNOB_SHARED_SPLITS, 2) * (long long)sms / base;
+        if (s > (blocks + least - 1) / least) s = (blocks + least - 1) / least;
+        s = s < 1 ? 1 : s > 64 ? 64 : s;
+        pl.keys_per_split = int((blocks + s - 1) / s) * kKeyBlock;
+        pl.splits = (a.prefix_len + pl.keys_per_split - 1) / pl.keys_per_split;
+    }
+    if (pl.prefix == PREFIX_TILES) {
         const int tokens = kBM / group, tiles = (a.batch + tokens - 1) / tokens, steps = (a.prefix_len + kBN - 1) / kBN;
         double best = 0;
-        for (int s = 1; s <= steps && s <= 32; ++s) {
+        const int forced_splits = tuning(KNOB_SHARED_SPLITS, 0);
+        for (int s = 1; s <= steps && s <= kMostSplits; ++s) {
+            if (forced_splits > 0 && s != (forced_splits < steps ? forced_splits : steps)) continue;
             for (int span = 1; span <= 2; ++span) {
                 if (span == 2 && tiles == 1) continue;
                 const long long items = (long long)(tiles + span - 1) / span * a.nKVHeads * s;
@@ -241,14 +404,22 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
                 if (best == 0 || t < best) { best = t; pl.splits = s; pl.span = span; }
             }
         }
-        const size_t rows = size_t(pl.splits) * a.batch * a.nQHeads;
-        pl.off_ml = (rows * a.D * 4 + 255) / 256 * 256;
-        pl.ws_bytes = pl.off_ml + (rows * 8 + 255) / 256 * 256;
     }
-    const long long keys = a.max_own + (pl.prefix_apart ? 0 : a.prefix_len);
+    if (pl.splits > 0) {
+        const size_t all = size_t(pl.splits) * a.batch * a.nQHeads;
+        pl.off_ml = (all * a.D * 4 + 255) / 256 * 256;
+        pl.ws_bytes = pl.off_ml + (all * 8 + 255) / 256 * 256;
+    }
+    const long long keys = a.max_own + (pl.prefix == PREFIX_HERE ? a.prefix_len : 0);
     pl.cluster = 1;
     while (pl.cluster < kMostOwnCluster && units * pl.cluster < 2 * sms && keys > 2 * kKeyBlock * kOwnWarps * pl.cluster) pl.cluster *= 2;
     return pl;
+}
+
+template <typename T, int D, int NT, int WK>
+int launch_prefix(const PrefixParams& p, int splits, cudaStream_t st) {
+    prefix_kernel<T, D, NT, WK><<<dim3(unsigned(splits), unsigned(p.nKVH * p.row_groups)), kOwnThreads, 0, st>>>(p);
+    return launched();
 }
 
 template <typename T, int D, int NT>
@@ -280,7 +451,17 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
     const int group = a.nQHeads / a.nKVHeads;
     float* part_o = static_cast<float*>(workspace);
     float* part_ml = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pl.off_ml);
-    if (pl.prefix_apart) {
+    if (pl.prefix == PREFIX_WARPS) {
+        PrefixParams p{};
+        p.q = q; p.K = Kp; p.V = Vp;
+        p.rows = a.batch * group; p.group = group; p.nKVH = a.nKVHeads; p.keys = a.prefix_len; p.keys_per_split = pl.keys_per_split;
+        p.row_groups = (p.rows + 8 * pl.nt * (kOwnWarps / pl.wk) - 1) / (8 * pl.nt * (kOwnWarps / pl.wk));
+        p.head = a.prefix_head; p.q_batch = a.q_batch; p.scale_log2 = scale_log2; p.part_o = part_o; p.part_ml = part_ml;
+        const int e = pl.nt == 1 ? launch_prefix<T, D, 1, 4>(p, pl.splits, st) : pl.wk == 4 ? launch_prefix<T, D, 2, 4>(p, pl.splits, st)
+                    : pl.wk == 2 ? launch_prefix<T, D, 2, 2>(p, pl.splits, st) : launch_prefix<T, D, 2, 1>(p, pl.splits, st);
+        if (e) return e;
+    }
+    if (pl.prefix == PREFIX_TILES) {
         PackedParams p{};
         p.Q = q; p.K = Kp; p.V = Vp;
         p.seqQ = a.batch; p.seqK = a.prefix_len; p.batch = 1;
@@ -290,13 +471,14 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
         p.part_o = part_o; p.part_ml = part_ml;
         if (int e = launch_packed<T, D, true>(p, a.dtype, st)) return e;
     }
+    const bool apart = pl.splits > 0;
     OwnParams w{};
     w.q = q; w.Kp = Kp; w.Vp = Vp; w.K = K; w.V = V; w.o = o; w.lengths = lengths;
     w.batch = a.batch; w.nKVH = a.nKVHeads; w.group = group; w.max_own = a.max_own; w.row_groups = (group + pl.rows - 1) / pl.rows;
-    w.prefix_here = pl.prefix_apart ? 0 : a.prefix_len; w.prefix_len = a.prefix_len;
+    w.prefix_here = pl.prefix == PREFIX_HERE ? a.prefix_len : 0; w.prefix_len = a.prefix_len;
     w.prefix_head = a.prefix_head; w.own_head = a.own_head; w.own_batch = a.own_batch; w.q_batch = a.q_batch; w.o_batch = a.o_batch;
-    w.scale_log2 = scale_log2; w.splits = pl.prefix_apart ? pl.splits : 0; w.part_o = part_o; w.part_ml = part_ml;
-    return pl.rows == 8 ? launch_own<T, D, 1>(w, pl.cluster, pl.prefix_apart, st) : launch_own<T, D, 2>(w, pl.cluster, pl.prefix_apart, st);
+    w.scale_log2 = scale_log2; w.splits = pl.splits; w.part_o = part_o; w.part_ml = part_ml;
+    return pl.rows == 8 ? launch_own<T, D, 1>(w, pl.cluster, apart, st) : launch_own<T, D, 2>(w, pl.cluster, apart, st);
 }
 
 int checked(const b200p_shared_args* args, b200p_shared_args* out) {

@@ -13,8 +13,8 @@
 namespace b200p {
 namespace {
 
-constexpr int kSegment = 8192;                   // tokens a CTA handles, a word of shared memory for each
 constexpr int kThreads = 256;
+constexpr int kSegment = 32 * kThreads;          // tokens a CTA handles, a word of shared memory for each
 constexpr int kMostBias = 1024;
 // A token's word: how often it was generated, and two flags.
 constexpr unsigned kInPrompt = 1u << 31, kBiased = 1u << 30, kCount = kBiased - 1;
@@ -41,52 +41,147 @@ __device__ __forceinline__ float adjusted(float x, unsigned word, int token, con
     return x;
 }
 
+__device__ __forceinline__ uint4 load_logits(const void* p) {        // may be the place that is written: not the read-only path
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+template <typename T> __device__ __forceinline__ T pick(const uint4& v, int e) { return reinterpret_cast<const T*>(&v)[e]; }
+template <typename T> __device__ __forceinline__ void put(uint4& v, int e, T x) { reinterpret_cast<T*>(&v)[e] = x; }
+
+// One CTA per (segment of the vocabulary, row).  HBM-bound: the logits are read and written once, 16 bytes at a time.  Their loads and
+// the mask's are issued first and are under way while the segment's part of the histories is counted: every CTA of a row reads
+// the row's whole histories (from L2, but for the first), keeps the ids of its segment and counts them in shared memory, so that no
+// count leaves the SM and nothing has to be cleared or merged.  Integer atomics: the order does not show.
+// Rows may start anywhere: places are counted from the last 16-byte boundary of `out` at or before the row, where a whole vector lies in
+// the row it is stored as one, and loaded as one if `in` lies the same way.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-logits_kernel(const LogitsParams p, const T* __restrict__ in, T* __restrict__ out) {
-    extern __shared__ unsigned words[];          // [kSegment]
+__global__ void __launch_bounds__(kThreads, 4)
+logits_kernel(const LogitsParams p, const T* in, T* out) {
+    constexpr int E = 16 / sizeof(T), VECS = kSegment / E / kThreads;
+    static_assert(VECS * E == 32, "a thread's places in one word");
+    extern __shared__ __align__(16) unsigned words[];               // [kSegment]
     const b200p_logits_args& a = p.a;
-    const int row = blockIdx.y, i0 = blockIdx.x * kSegment, n = min(kSegment, a.vocab - i0);
-    for (int i = threadIdx.x; i < n; i += kThreads) words[i] = 0;
-    __syncthreads();
-    auto length = [&](const int* lengths, int stride, int most) { return lengths ? min(max(lengths[size_t(row) * stride], 0), most) : most; };
-    if (a.prompt) {
-        const int m = length(a.prompt_lengths, p.prompt_ls, a.prompt_max);
-        for (int i = threadIdx.x; i < m; i += kThreads) {
-            const unsigned t = unsigned(a.prompt[size_t(row) * a.prompt_max + i]) - unsigned(i0);
-            if (t < unsigned(n)) atomicOr(&words[t], kInPrompt);
-        }
-    }
-    if (a.tokens) {
-        const int m = length(a.token_lengths, p.token_ls, a.tokens_max);
-        for (int i = threadIdx.x; i < m; i += kThreads) {
-            const unsigned t = unsigned(a.tokens[size_t(row) * a.tokens_max + i]) - unsigned(i0);
-            if (t < unsigned(n)) atomicAdd(&words[t], 1u);
-        }
-    }
-    RowRules r{a.repetition ? a.repetition[row] : 1.f, a.presence ? a.presence[row] : 0.f, a.frequency ? a.frequency[row] : 0.f,
-               a.bias_ids + size_t(row) * a.bias_n, a.bias_values + size_t(row) * a.bias_n, a.bias_n};
-    for (int i = threadIdx.x; i < a.bias_n; i += kThreads) {
-        const unsigned t = unsigned(r.bias_ids[i]) - unsigned(i0);
-        if (t < unsigned(n)) atomicOr(&words[t], kBiased);
-    }
-    __syncthreads();
+    const int row = blockIdx.y, V = a.vocab;
+    const T* const x = in + size_t(row) * a.in_stride;
+    T* const y = out + size_t(row) * a.out_stride;
+    const int before = int(reinterpret_cast<uintptr_t>(y) % 16 / sizeof(T));
+    const bool alike = reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T) == unsigned(before);
+    const int i0 = int(blockIdx.x) * kSegment - before;             // the segment's first token (negative: what lies before the row)
+    if (i0 >= V) return;                                            // the grid has room for a row that starts behind a boundary
+    const bool whole = alike && i0 >= 0 && i0 + kSegment <= V;      // vectors only
     const int which = a.mask ? (a.mask_rows ? a.mask_rows[row] : row) : -1;
-    const unsigned* mask = which >= 0 && which < a.n_masks ? a.mask + size_t(which) * ((a.vocab + 31) / 32) : nullptr;
-    const T* x = in + size_t(row) * a.in_stride;
-    T* y = out + size_t(row) * a.out_stride;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int token = i0 + i;
-        float v = adjusted(to_float(x[token]), words[i], token, r);
-        if (mask && !(mask[token >> 5] >> (token & 31) & 1u)) v = -INFINITY;
-        y[token] = from_float<T>(v);
+    const unsigned* const mask = which >= 0 && which < a.n_masks ? a.mask + size_t(which) * ((V + 31) / 32) : nullptr;
+    auto token_of = [&](int k) { return i0 + (k * kThreads + int(threadIdx.x)) * E; };     // the vector's first
+    uint4 v[VECS];
+    if (whole) {
+        #pragma unroll
+        for (int k = 0; k < VECS; ++k) v[k] = load_logits(x + token_of(k));
+    } else {
+        #pragma unroll
+        for (int k = 0; k < VECS; ++k) {
+            const int t = token_of(k);
+            if (alike && t >= 0 && t + E <= V) v[k] = load_logits(x + t);
+            else {
+                #pragma unroll
+                for (int e = 0; e < E; ++e) if (t + e >= 0 && t + e < V) put<T>(v[k], e, x[t + e]);
+            }
+        }
+    }
+    unsigned allowed = ~0u;                                         // of this thread's 32 places
+    if (mask) {
+        allowed = 0;
+        if (whole && before == 0) {                                 // a vector's bits in one word
+            #pragma unroll
+            for (int k = 0; k < VECS; ++k) allowed |= (mask[token_of(k) >> 5] >> (token_of(k) & 31) & ((1u << E) - 1)) << (k * E);
+        } else {
+            #pragma unroll
+            for (int k = 0; k < VECS; ++k) {
+                const int t = token_of(k);
+                if (t + E <= 0 || t >= V) continue;
+                const int f = max(t, 0), l = min(t + E, V) - 1;
+                const unsigned lo = mask[f >> 5], hi = (l >> 5) != (f >> 5) ? mask[l >> 5] : 0u;
+                allowed |= (__funnelshift_r(lo, hi, f & 31) << (f - t) & ((1u << E) - 1)) << (k * E);
+            }
+        }
+    }
+    // The lists' first ids, ahead of their lengths: up to a row's end they are there, whether they count or not.
+    const int* const prompt = a.prompt + size_t(row) * a.prompt_max; const int* const tokens = a.tokens + size_t(row) * a.tokens_max;
+    const int* const biased = a.bias_ids + size_t(row) * a.bias_n;
+    constexpr int P0 = 4, T0 = 2, B0 = 1;
+    int id_p[P0], id_t[T0], id_b[B0];
+    auto first_ids = [&](auto& id, const int* ids, int n) {
+        #pragma unroll
+        for (int u = 0; u < int(sizeof(id) / 4); ++u) { const int i = u * kThreads + int(threadIdx.x); id[u] = i < n ? ids[i] : -1; }
+    };
+    first_ids(id_p, prompt, a.prompt ? a.prompt_max : 0);
+    first_ids(id_t, tokens, a.tokens ? a.tokens_max : 0);
+    first_ids(id_b, biased, a.bias_n);
+    auto length = [&](const int* ids, const int* lengths, int stride, int most) { return !ids ? 0 : lengths ? min(max(lengths[size_t(row) * stride], 0), most) : most; };
+    const int n_prompt = length(a.prompt, a.prompt_lengths, p.prompt_ls, a.prompt_max), n_tokens = length(a.tokens, a.token_lengths, p.token_ls, a.tokens_max);
+    const RowRules r{a.repetition ? a.repetition[row] : 1.f, a.presence ? a.presence[row] : 0.f, a.frequency ? a.frequency[row] : 0.f,
+                     biased, a.bias_values + size_t(row) * a.bias_n, a.bias_n};
+    unsigned touched = 0;                                           // of this thread's places
+    if (n_prompt + n_tokens + a.bias_n > 0) {                       // the same in all threads
+        #pragma unroll
+        for (int i = 0; i < kSegment / 4 / kThreads; ++i) reinterpret_cast<uint4*>(words)[i * kThreads + threadIdx.x] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        const int low = max(i0, 0);                                 // the segment's ids: low ... low + range - 1
+        const unsigned range = unsigned(min(i0 + kSegment, V) - low);
+        auto each = [&](auto& first, const int* ids, int n, auto&& mark) {
+            constexpr int F = int(sizeof(first) / 4), U = 4;        // U loads in flight
+            #pragma unroll
+            for (int u = 0; u < F; ++u) if (u * kThreads + int(threadIdx.x) < n && unsigned(first[u] - low) < range) mark(&words[first[u] - i0]);
+            for (int i = F * kThreads + int(threadIdx.x); i < n; i += U * kThreads) {
+                int id[U];
+                #pragma unroll
+                for (int u = 0; u < U; ++u) id[u] = i + u * kThreads < n ? ids[i + u * kThreads] : -1;
+                #pragma unroll
+                for (int u = 0; u < U; ++u) if (unsigned(id[u] - low) < range) mark(&words[id[u] - i0]);
+            }
+        };
+        each(id_p, prompt, n_prompt, [](unsigned* w) { atomicOr(w, kInPrompt); });
+        each(id_t, tokens, n_tokens, [](unsigned* w) { atomicAdd(w, 1u); });
+        each(id_b, biased, a.bias_n, [](unsigned* w) { atomicOr(w, kBiased); });
+        __syncthreads();
+        #pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const uint4 w = *reinterpret_cast<const uint4*>(&words[(q * 4 / E * kThreads + int(threadIdx.x)) * E + q * 4 % E]);
+            touched |= (w.x ? 1u : 0u) << (4 * q) | (w.y ? 2u : 0u) << (4 * q) | (w.z ? 4u : 0u) << (4 * q) | (w.w ? 8u : 0u) << (4 * q);
+        }
+        touched &= allowed;                                         // a masked one stays masked
+    }
+    // All logits out, but for the masked ones as they came in.  Those that the rules touch are done in a loop of its own: the rules
+    // inlined at every place are more code than the instruction cache holds (256 rows of 128000: 141 us, so 93).
+    const T none = from_float<T>(-INFINITY);
+    #pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+        if (mask) {
+            #pragma unroll
+            for (int e = 0; e < E; ++e) if (!(allowed >> (k * E + e) & 1u)) put<T>(v[k], e, none);
+        }
+        const int t = token_of(k);
+        if (whole || (t >= 0 && t + E <= V)) *reinterpret_cast<uint4*>(y + t) = v[k];
+        else {
+            #pragma unroll
+            for (int e = 0; e < E; ++e) if (t + e >= 0 && t + e < V) y[t + e] = pick<T>(v[k], e);
+        }
+    }
+    for (; touched; touched &= touched - 1) {
+        const int b = __ffs(touched) - 1, place = (b / E * kThreads + int(threadIdx.x)) * E + b % E, t = i0 + place;
+        T z = pick<T>(v[0], 0);                                     // the value is still in a register: found by comparisons, not read again
+        #pragma unroll
+        for (int i = 1; i < 32; ++i) if (i == b) z = pick<T>(v[i / E], i % E);
+        y[t] = from_float<T>(adjusted(to_float(z), words[place], t, r));
     }
 }
 
 template <typename T>
 int launch(const void* in, void* out, const LogitsParams& p, cudaStream_t st) {
-    const dim3 grid(unsigned((p.a.vocab + kSegment - 1) / kSegment), unsigned(p.a.rows));
-    logits_kernel<T><<<grid, kThreads, kSegment * sizeof(unsigned), st>>>(p, static_cast<const T*>(in), static_cast<T*>(out));
+    const long long places = (long long)p.a.vocab + 16 / (long long)sizeof(T) - 1;
+    constexpr int kBytes = kSegment * int(sizeof(unsigned));
+    if (int e = allow_dynamic_smem(reinterpret_cast<const void*>(logits_kernel<T>), kBytes)) return e;
+    logits_kernel<T><<<dim3(unsigned((places + kSegment - 1) / kSegment), unsigned(p.a.rows)), kThreads, kBytes, st>>>(p, static_cast<const T*>(in), static_cast<T*>(out));
     return launched();
 }
 

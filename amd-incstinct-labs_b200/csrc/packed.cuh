@@ -65,13 +65,15 @@ __device__ __forceinline__ void packed_walk(const PackedParams& p, Publish&& pub
         const int x = behind - (m - n);                         // a block whose last token is behind x sees more than `behind` keys
         return x < 0 ? 0 : min(nb, x / block);
     };
-    int levels = 0, chunk_levels = 0;                           // lane c: of chunk c
+    int levels = 0, chunk_levels = 0, blocks = 0;               // lane c: of chunk c
     for (int c = 0; c < chunks; ++c) {
         load(c);
+        blocks += (n + block - 1) / block;
         const int most = __reduce_max_sync(kAll, n == 0 ? 0 : max(1, (m + kBN - 1) / kBN));
         if (lane == c) chunk_levels = most;
         levels = max(levels, most);
     }
+    blocks = __reduce_add_sync(kAll, blocks);
     const int per = p.nKVH * p.splits;
     int level = levels, c = 0, at = -1;                         // at: the chunk that is loaded
     if (chunks == 1) at = 0;
@@ -81,6 +83,7 @@ __device__ __forceinline__ void packed_walk(const PackedParams& p, Publish&& pub
         const int entry = id / per, rest = id - entry * per;
         PackedItem w{};
         w.kvh = -1;
+        if (entry >= blocks) level = 0;                         // no more
         while (level > 0) {
             if (total < 0) {
                 if (c < 32 && __shfl_sync(kAll, chunk_levels, c & 31) < level) total = 0;
@@ -96,7 +99,10 @@ __device__ __forceinline__ void packed_walk(const PackedParams& p, Publish&& pub
             }
             if (entry - base < total) break;
             base += total; total = -1;
-            if (++c == chunks) { c = 0; --level; }
+            if (chunks == 1) {                                  // on to the next level that a block has: that of the last one before `first`
+                const int before = min(m, p.causal ? m - n + first * block : m);
+                level = __reduce_max_sync(kAll, first == 0 ? 0 : max(1, (before + kBN - 1) / kBN));
+            } else if (++c == chunks) { c = 0; --level; }
         }
         if (level > 0) {
             const int within = entry - base;

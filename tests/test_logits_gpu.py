@@ -33,7 +33,9 @@ def same(torch, got, want, bound):
 @pytest.mark.parametrize("kind", ["float32", "bfloat16", "float16"])
 @pytest.mark.parametrize("rows,vocab,prompt,tokens,bias,masks", [
     (1, 1, 3, 2, 1, 1), (1, 33, 5, 5, 3, 2), (3, 1000, 40, 20, 5, 2), (2, 8191, 300, 0, 0, 0), (4, 8193, 0, 300, 0, 3), (2, 20001, 7, 7, 64, 0), (5, 32000, 500, 100, 0, 1),
-    (3, 1234, 0, 0, 0, 2), (2, 50001, 0, 0, 10, 0), (1, 4096, 3000, 5000, 1024, 1)])
+    (3, 1234, 0, 0, 0, 2), (2, 50001, 0, 0, 10, 0), (1, 4096, 3000, 5000, 1024, 1),
+    # about a segment's end, whichever way the rows lie
+    (3, 8185, 50, 60, 4, 1), (2, 8190, 50, 60, 4, 1), (2, 8192, 50, 60, 4, 1), (3, 16383, 900, 1500, 300, 2)])
 def test_rules(b200p, torch_cuda, rows, vocab, prompt, tokens, bias, masks, kind):
     torch = torch_cuda
     x = request(torch, rows, vocab, prompt, tokens, bias, masks, seed=vocab)
