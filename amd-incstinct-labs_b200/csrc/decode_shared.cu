@@ -62,7 +62,7 @@ __device__ __forceinline__ float weight_of(float m, float most) { return exp2f(m
 // them, for K and Q alike; V's rows are paired up by byte permutes.  No shared memory and no barrier stands between the loads and the
 // products; a warp has 8 KB (heads of 128) in flight.  Rows past the run's end are not read: their registers are zero.
 // Lane (g, t4) = (lane / 4, lane % 4).
-template <typename T, int D, int NT, bool CACHED> struct KeyWalk {
+template <typename T, int D, int NT> struct KeyWalk {
     static constexpr int KC = D / 32, VC = D / 64, R = 8 * NT;
     uint4 qf[NT][KC];                                     // row n * 8 + g, columns 32 c + 8 t4 ..
     uint4 kf[2][KC], vf[4][VC];                           // keys g, g + 8, the same columns; keys 2 t4, + 1, + 8, + 9, columns 64 c + 8 g ..
@@ -80,8 +80,7 @@ template <typename T, int D, int NT, bool CACHED> struct KeyWalk {
     }
     static __device__ __forceinline__ uint4 load16(const T* p) {
         uint4 v;
-        if constexpr (CACHED) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-        else asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
         return v;
     }
     // row: this lane's row (n * 8 + g) or null
@@ -181,71 +180,6 @@ template <typename T, int D, int NT, bool CACHED> struct KeyWalk {
     }
 };
 
-// The prefix for batches whose rows are few (plan_shared): warps of a CTA that share the keys of its split have other query rows
-// (K and V then come from L1 for all but the first of them), WK of them take every WK-th block of 16 keys for the same rows and
-// meet in shared memory.  Small CTAs, so that the next launch's find room beside them and read the sequences' own keys meanwhile.
-struct PrefixParams {
-    const void *q, *K, *V;
-    int rows, group, nKVH, keys, keys_per_split, row_groups;     // rows: batch * group, of a key head; row_groups: CTAs over them
-    long long head, q_batch;
-    float scale_log2;
-    float *part_o, *part_ml;
-};
-template <typename T, int D, int NT, int WK>
-__global__ void __launch_bounds__(kOwnThreads, NT == 1 ? 4 : D == 64 ? 3 : 2)
-prefix_kernel(const PrefixParams p) {
-    constexpr int WR = kOwnWarps / WK, R = 8 * NT;
-    __shared__ __align__(16) float s_o[WK > 1 ? kOwnWarps : 1][R][D + 4];
-    __shared__ float s_ml[kOwnWarps][R][2];
-    griddep_launch_dependents();
-    const int warp = threadIdx.x / 32, split = blockIdx.x, kvh = blockIdx.y / p.row_groups, rg = blockIdx.y % p.row_groups;
-    const int row0 = (rg * WR + warp / WK) * R, nQH = p.nKVH * p.group;
-    KeyWalk<T, D, NT, true> w;
-    #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int row = row0 + n * 8 + w.g, b = row / p.group;
-        w.load_q(n, row < p.rows ? static_cast<const T*>(p.q) + b * p.q_batch + (long long)(kvh * p.group + row - b * p.group) * D : nullptr);
-    }
-    const int k0 = split * p.keys_per_split, keys = min(p.keys_per_split, p.keys - k0), blocks = (keys + kKeyBlock - 1) / kKeyBlock;
-    const T* const K = static_cast<const T*>(p.K) + kvh * p.head + (long long)k0 * D; const T* const V = static_cast<const T*>(p.V) + kvh * p.head + (long long)k0 * D;
-    if (row0 < p.rows) {
-        int j = warp % WK;
-        if (j < blocks) { w.load_k(K + j * kKeyBlock * D, keys - j * kKeyBlock); w.load_v(V + j * kKeyBlock * D, keys - j * kKeyBlock); }
-        for (; j < blocks; j += WK) {
-            const int next = (j + WK) * kKeyBlock;
-            w.step(keys - j * kKeyBlock, p.scale_log2, [&] { if (next < keys) w.load_k(K + (long long)next * D, keys - next); });
-            if (next < keys) w.load_v(V + (long long)next * D, keys - next);
-        }
-    }
-    // row r of the partial results: [split][sequence][head]
-    auto part_row = [&](int row) { const int b = row / p.group; return (size_t(split) * (p.rows / p.group) + b) * nQH + kvh * p.group + row - b * p.group; };
-    if constexpr (WK == 1) {
-        w.result([&](int row, float m, float l) { if (row0 + row < p.rows) *reinterpret_cast<float2*>(&p.part_ml[2 * part_row(row0 + row)]) = make_float2(m, l); },
-                 [&](int row, int d, float4 v) { if (row0 + row < p.rows) *reinterpret_cast<float4*>(&p.part_o[part_row(row0 + row) * D + d]) = v; });
-    } else {
-        w.result([&](int row, float m, float l) { s_ml[warp][row][0] = m; s_ml[warp][row][1] = l; }, [&](int row, int d, float4 v) { *reinterpret_cast<float4*>(&s_o[warp][row][d]) = v; });
-        __syncthreads();
-        for (int i = threadIdx.x; i < WR * R * (D / 4); i += kOwnThreads) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4, w0 = r / R * WK, in = r % R, row = rg * WR * R + r;
-            if (row >= p.rows) break;
-            float most = -INFINITY, sum = 0.f;
-            #pragma unroll
-            for (int k = 0; k < WK; ++k) most = fmaxf(most, s_ml[w0 + k][in][0]);
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            #pragma unroll
-            for (int k = 0; k < WK; ++k) {
-                const float f = weight_of(s_ml[w0 + k][in][0], most);
-                const float4 v = *reinterpret_cast<const float4*>(&s_o[w0 + k][in][d]);
-                sum += f * s_ml[w0 + k][in][1];
-                x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
-            }
-            const size_t at = part_row(row);
-            *reinterpret_cast<float4*>(&p.part_o[at * D + d]) = x;
-            if (d == 0) *reinterpret_cast<float2*>(&p.part_ml[2 * at]) = make_float2(most, sum);
-        }
-    }
-}
-
 // The sequences' own keys (and the prefix's where it has no launch of its own), and the merge.  One cluster of `gridDim.x` CTAs per
 // (sequence, key head, 8 * NT query rows); a warp takes every (warps of the cluster)-th block of 16 keys.
 template <typename T, int D, int NT>
@@ -260,7 +194,7 @@ own_kernel(const OwnParams p) {
     const int ctas = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y / p.row_groups, r0 = (blockIdx.y % p.row_groups) * R, b = blockIdx.z;
     const int rows = min(R, p.group - r0), nQH = p.nKVH * p.group, head0 = kvh * p.group + r0;
 
-    KeyWalk<T, D, NT, false> w;
+    KeyWalk<T, D, NT> w;
     const int prefix_blocks = (p.prefix_here + kKeyBlock - 1) / kKeyBlock, stride = ctas * kOwnWarps;
     const T* const own_k = static_cast<const T*>(p.K) + b * p.own_batch + kvh * p.own_head; const T* const own_v = static_cast<const T*>(p.V) + b * p.own_batch + kvh * p.own_head;
     const T* const prefix_k = static_cast<const T*>(p.Kp) + kvh * p.prefix_head; const T* const prefix_v = static_cast<const T*>(p.Vp) + kvh * p.prefix_head;
@@ -358,11 +292,10 @@ own_kernel(const OwnParams p) {
 }
 
 // How a call is run.
-enum PrefixKind { PREFIX_NONE, PREFIX_HERE, PREFIX_WARPS, PREFIX_TILES };       // no keys; by own_kernel; prefix_kernel; the tcgen05 kernel
+enum PrefixKind { PREFIX_NONE, PREFIX_HERE, PREFIX_TILES };       // no keys; by own_kernel, per sequence; a launch of the tcgen05 kernel
 struct SharedPlan {
     int prefix;
-    int splits, span;            // of the prefix's launch; span: tiles of an item (PREFIX_TILES)
-    int keys_per_split, wk, nt;  // PREFIX_WARPS
+    int splits, span;            // PREFIX_TILES: of its launch; span: tiles of an item
     int cluster, rows;           // CTAs and query rows (8 or 16) of a unit of the second launch
     size_t off_ml, ws_bytes;
 };
@@ -370,26 +303,13 @@ struct SharedPlan {
 SharedPlan plan_shared(const b200p_shared_args& a) {
     SharedPlan pl{};
     const int sms = sm_count() > 0 ? sm_count() : 148, group = a.nQHeads / a.nKVHeads;
-    const long long rows = (long long)a.batch * group, blocks = (a.prefix_len + kKeyBlock - 1) / kKeyBlock;
     pl.rows = group <= 8 ? 8 : 16;
     const long long units = (long long)a.batch * a.nKVHeads * ((group + pl.rows - 1) / pl.rows);
     if (a.prefix_len == 0) pl.prefix = PREFIX_NONE;
     else if ((long long)a.batch * a.prefix_len <= 4096) pl.prefix = PREFIX_HERE;
-    else pl.prefix = rows * a.prefix_len * a.nKVHeads * a.D <= (1LL << 32) ? PREFIX_WARPS : PREFIX_TILES;
+    else pl.prefix = PREFIX_TILES;
     const int forced = tuning(KNOB_SHARED_PREFIX, 0);
     if (a.prefix_len > 0 && forced >= PREFIX_HERE && forced <= PREFIX_TILES) pl.prefix = forced;
-    if (pl.prefix == PREFIX_WARPS) {
-        pl.nt = rows <= 8 ? 1 : 2;
-        const long long warps = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
-        const int wr = warps >= 3 ? 4 : int(warps);
-        pl.wk = kOwnWarps / wr;
-        const long long base = a.nKVHeads * ((warps + wr - 1) / wr), least = 2 * pl.wk;        // blocks of a split
-        long long s = tuning(KNOB_SHARED_SPLITS, 2) * (long long)sms / base;
-        if (s > (blocks + least - 1) / least) s = (blocks + least - 1) / least;
-        s = s < 1 ? 1 : s > 64 ? 64 : s;
-        pl.keys_per_split = int((blocks + s - 1) / s) * kKeyBlock;
-        pl.splits = (a.prefix_len + pl.keys_per_split - 1) / pl.keys_per_split;
-    }
     if (pl.prefix == PREFIX_TILES) {
         const int tokens = kBM / group, tiles = (a.batch + tokens - 1) / tokens, steps = (a.prefix_len + kBN - 1) / kBN;
         double best = 0;
@@ -414,12 +334,6 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
     pl.cluster = 1;
     while (pl.cluster < kMostOwnCluster && units * pl.cluster < 2 * sms && keys > 2 * kKeyBlock * kOwnWarps * pl.cluster) pl.cluster *= 2;
     return pl;
-}
-
-template <typename T, int D, int NT, int WK>
-int launch_prefix(const PrefixParams& p, int splits, cudaStream_t st) {
-    prefix_kernel<T, D, NT, WK><<<dim3(unsigned(splits), unsigned(p.nKVH * p.row_groups)), kOwnThreads, 0, st>>>(p);
-    return launched();
 }
 
 template <typename T, int D, int NT>
@@ -451,16 +365,6 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
     const int group = a.nQHeads / a.nKVHeads;
     float* part_o = static_cast<float*>(workspace);
     float* part_ml = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pl.off_ml);
-    if (pl.prefix == PREFIX_WARPS) {
-        PrefixParams p{};
-        p.q = q; p.K = Kp; p.V = Vp;
-        p.rows = a.batch * group; p.group = group; p.nKVH = a.nKVHeads; p.keys = a.prefix_len; p.keys_per_split = pl.keys_per_split;
-        p.row_groups = (p.rows + 8 * pl.nt * (kOwnWarps / pl.wk) - 1) / (8 * pl.nt * (kOwnWarps / pl.wk));
-        p.head = a.prefix_head; p.q_batch = a.q_batch; p.scale_log2 = scale_log2; p.part_o = part_o; p.part_ml = part_ml;
-        const int e = pl.nt == 1 ? launch_prefix<T, D, 1, 4>(p, pl.splits, st) : pl.wk == 4 ? launch_prefix<T, D, 2, 4>(p, pl.splits, st)
-                    : pl.wk == 2 ? launch_prefix<T, D, 2, 2>(p, pl.splits, st) : launch_prefix<T, D, 2, 1>(p, pl.splits, st);
-        if (e) return e;
-    }
     if (pl.prefix == PREFIX_TILES) {
         PackedParams p{};
         p.Q = q; p.K = Kp; p.V = Vp;

@@ -184,11 +184,14 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
     uint64_t* o_free  = q_empty + 1;          // [2] the tile's epilogue has read O out of tensor memory
     uint64_t* item_full  = o_free + 2;        // [2] ring of work-item ids
     uint64_t* item_empty = item_full + 2;     // [2]
+    uint64_t* answer_bar = item_empty + 2;    // [1] PACKED: an answer of the launch control
+    uint64_t* ask_next = answer_bar + 1;      // [1] PACKED: time to look for the next item
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_failed;
     __shared__ int s_item[2];
     using Item = std::conditional_t<PACKED, PackedItem, PrefillItem>;
     __shared__ std::conditional_t<PACKED, PackedItem, int> s_packed[2];
+    __shared__ __align__(16) uint4 s_answer[1];
 
     constexpr int kMmaWarp = 8 * RS, kTmaWarp = 8 * RS + 1, kWalkWarp = 8 * RS + 2;
     constexpr int kItemReaders = 2 * kBM + 1 + PACKED;         // every softmax thread + the MMA thread; PACKED: + the TMA thread
@@ -205,6 +208,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
             dme::mbar_init(&o_done[t], 1); dme::mbar_init(&o_free[t], kBM);
             dme::mbar_init(&item_full[t], 1); dme::mbar_init(&item_empty[t], kItemReaders);
         }
+        if constexpr (PACKED) { dme::mbar_init(answer_bar, 1); dme::mbar_init(ask_next, 1); }
         dme::mbar_init_fence();
     }
     if (warp == kMmaWarp) { tc::tmem_alloc(&s_tmem_base, 512); tc::tmem_relinquish(); }
@@ -220,19 +224,24 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
     // other roles read them there.  All barrier phases run on across items, so the next item's Q, K_0 and
     // first Q.K^T are under way while the softmax warps still normalise and store the previous item's O.
     // PACKED: a warp of its own (kWalkWarp) finds the items from the sequences' lengths, which are known on the device only, and
-    // publishes them whole; a CTA's items are a fixed share of the launch's, heaviest first, so no counter has to be cleared.
+    // publishes them whole.
     int* const abort_word = [&] { if constexpr (PACKED) return &s_failed; else return p.status; }();     // PACKED: no CTA waits for another
     auto read_item = [&](int it, Item& w) -> int {             // behind item_full: the CTA's it-th item; its id, or negative: there are no more
-        if constexpr (PACKED) { w = s_packed[it & 1]; return w.kvh; }
+        if constexpr (PARTIAL) {                               // known without looking: every role finds them itself
+            const int id = int(blockIdx.x) + it * int(gridDim.x);
+            if (id >= p.items) return -1;
+            w = packed_split(p, id);
+            return id;
+        } else if constexpr (PACKED) { w = s_packed[it & 1]; return w.kvh; }
         else {
             const int id = *reinterpret_cast<volatile int*>(&s_item[it & 1]);
             return id;
         }
     };
     auto next_item = [&](int it, Item& w) -> int {             // consumer side
-        if (!dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word)) return -2;
+        if (!PARTIAL && !dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word)) return -2;
         const int id = read_item(it, w);
-        dme::mbar_arrive(&item_empty[it & 1]);
+        if (!PARTIAL) dme::mbar_arrive(&item_empty[it & 1]);
         return id;
     };
 
@@ -256,7 +265,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                 if constexpr (PACKED) {
                     const int id = next_item(it, w);
                     if (id < 0) { ok = id != -2; break; }
-                    if (w.nmax == 0) continue;                   // rows without keys: only zeros to write
+                    if (w.nmax == 0) { dme::mbar_arrive(ask_next); continue; }      // rows without keys: only zeros to write
                     if (worked >= 1 && !dme::wait(q_empty, uint32_t((worked - 1) & 1), abort_word)) { ok = false; break; }
                     ++worked;
                     dme::mbar_arrive_expect_tx(q_full, uint32_t((w.n[0] > 0) + (w.n[1] > 0)) * Sh::QK_SUB * uint32_t(p.tokens * p.group) * 128u);
@@ -290,6 +299,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                         else                  dme::copy_tile_4d(dst, &mapK, sb * 64, (w.first + j) * kBN, w.kvh, w.b, &k_full[kr.stage]);
                     }
                     kr.advance(); ++kloads;
+                    if constexpr (PACKED) if (j == max(w.nmax - kAskAhead, 0)) dme::mbar_arrive(ask_next);
                     if (vloads >= VST && !dme::wait(&v_empty[vr.stage], vr.phase ^ 1u, abort_word)) { ok = false; break; }
                     dme::mbar_arrive_expect_tx(&v_full[vr.stage], Sh::V_BYTES);
                     for (int sb = 0; sb < Sh::V_SUB; ++sb) {
@@ -338,11 +348,11 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         int worked = 0;                // PACKED: earlier items with keys: phase of q_full
         bool ok = true;
         for (int it = 0; ok; ++it) {
-            if (!wait(&item_full[it & 1], uint32_t((it >> 1) & 1))) { ok = false; break; }
+            if (!PARTIAL && !wait(&item_full[it & 1], uint32_t((it >> 1) & 1))) { ok = false; break; }
             Item w;
             const int id = __shfl_sync(0xffffffffu, read_item(it, w), 0);
             if constexpr (PACKED) __syncwarp();                  // all lanes have read the item
-            if (tc::elect_one()) dme::mbar_arrive(&item_empty[it & 1]);
+            if (!PARTIAL) { if (tc::elect_one()) dme::mbar_arrive(&item_empty[it & 1]); }
             __syncwarp();
             if (id < 0) break;
             if constexpr (PACKED) {
@@ -427,17 +437,20 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
             cs0 += n0; cs1 += n1; co0 += n0 > 0; co1 += n1 > 0;
         }
         if (!ok && lane == 0) atomicExch(&s_failed, 1);
-      } else if (PACKED && warp == kWalkWarp) {
-        if constexpr (PACKED) {
+      } else if (PACKED && !PARTIAL && warp == kWalkWarp) {
+        if constexpr (PACKED && !PARTIAL) {
             bool ok = true;
-            packed_walk(p, [&](int it, const PackedItem& w) -> bool {
+            const bool fine = packed_walk(p, s_answer, answer_bar, [&](int it, const PackedItem& w) -> bool {
                 if (it >= 2) ok = dme::wait(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1), abort_word);
                 ok = __all_sync(0xffffffffu, ok) != 0;
                 if (ok && lane == 0) { s_packed[it & 1] = w; dme::mbar_arrive(&item_full[it & 1]); }
                 __syncwarp();
+                // a next item is asked for with this one's last steps ahead (kAskAhead): what a busy CTA holds is work that idle ones
+                // miss (6 portions of prompts, 184 items: 157 us when asked for at an item's begin)
+                if (ok && w.kvh >= 0) ok = __all_sync(0xffffffffu, dme::wait(ask_next, uint32_t(it & 1), abort_word)) != 0;
                 return ok;
             });
-            if (!ok && lane == 0) atomicExch(&s_failed, 1);
+            if (!(ok && fine) && lane == 0) atomicExch(&s_failed, 1);
         }
       }
     } else {
@@ -580,7 +593,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                 tc::wait_ld();
                 tc::fence_before_sync();
                 dme::mbar_arrive(&o_free[t]);
-                packed_epilogue<T, Sh>(p, w, v, m_used, l, nt, q0t, row_token, live, r, stage, issuer, tile_sync, [&](bool mine) { return !all_of_tile(!mine); }, &mapO);
+                packed_epilogue<T, Sh>(p, w, v, m_used, l, nt, q0t, row_token, live, r);
             } else if (live) packed_no_keys<T, Sh>(p, w, row, r - row_token * p.group);
           } else if (nt > 0) {
             tc::fence_after_sync();
