@@ -4,13 +4,14 @@
 //
 // Softmax over both parts is the merge of what each part gives (m: maximum, l: sum, O: weighted sum of values):
 //   m = max m_i;  l = sum l_i 2^(m_i - m);  O = sum O_i 2^(m_i - m) / l.
-// Two launches:
+// Three launches:
 //  1. the prefix, for the whole batch: the query rows of a key head are ONE matrix of batch * group rows, so this is the tcgen05
 //     prefill kernel (packed.cuh) over one "sequence" of `batch` tokens without a mask, its keys split so that all SMs have work;
 //     (m, l, O) of every split go to the workspace in fp32.  Each tile of the prefix is read once per 256 rows.
-//  2. the sequences' own keys, and the merge: HBM-bound, every byte of the caches is read once (own_kernel below).  It is a
-//     programmatic dependent of the first launch and waits for it only ahead of the merge.
-// A prefix that is small for its batch is cheaper read per sequence (from L2) by the second kernel alone.
+//  2. the sequences' own keys (own_kernel): HBM-bound, every byte of the caches is read once.  A programmatic dependent that
+//     waits for nothing: its CTAs run wherever the first launch leaves room.
+//  3. the merge (merge_kernel).
+// A prefix that is small for its batch is cheaper read per sequence (from L2), by own_kernel, which then is the only launch.
 // ---------------------------------------------------------------------------
 #include "packed_launch.cuh"
 
@@ -21,18 +22,20 @@ constexpr int kOwnWarps = 4;
 constexpr int kOwnThreads = kOwnWarps * 32;
 constexpr int kKeyBlock = 16;                    // keys of a warp's step
 constexpr int kMostOwnCluster = 8;
-constexpr int kMostSplits = 160;                 // of the prefix: one for each SM, for a single key head
+constexpr int kMostSplits = 152;                 // of the prefix: one for each SM, for a single key head
+constexpr int kMostParts = kMostSplits + kMostOwnCluster;
 
 struct OwnParams {
     const void *q, *Kp, *Vp, *K, *V;
     void* o;
     const int* lengths;
     int batch, nKVH, group, max_own, row_groups;
-    int prefix_here, prefix_len;                 // keys of the prefix that this kernel reads itself; all of the prefix
+    int prefix_here;                             // keys of the prefix that this kernel reads itself
     long long prefix_head, own_head, own_batch, q_batch, o_batch;
     float scale_log2;
-    int splits;                                  // of the prefix, in the workspace
-    const float *part_o, *part_ml;               // [splits][batch][nQH][D], [..][2]
+    int apart;                                   // 1: results go to the workspace, as parts `first_part` + the CTA's place in its unit
+    int first_part;
+    float *part_o, *part_ml;                     // [part][batch][nQH][D], not divided; [..][2]: maximum in log2 units, sum
 };
 
 __device__ __forceinline__ uint32_t transposed_8x8(uint32_t x) {
@@ -56,6 +59,20 @@ __device__ __forceinline__ float4 load_cluster_f32x4(uint32_t smem, uint32_t cta
 }
 __device__ __forceinline__ float weight_of(float m, float most) { return exp2f(m - (most == -INFINITY ? 0.f : most)); }
 
+// 2^(m_i - m) of this lane's part, m the maximum over the warp, and 1 / sum of 2^(m_i - m) l_i.  A sum of 0 is a part without keys, whose O
+// means nothing.
+__device__ __forceinline__ float part_weight(float2 ml, float& inv) {
+    float most = ml.x;
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    const float f = ml.y == 0.f ? 0.f : weight_of(ml.x, most);
+    float sum = f * ml.y;
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    inv = 1.f / sum;
+    return f;
+}
+
 // Up to 8 * NT query rows against blocks of 16 keys by one warp.  A step is S^T = K Q^T and O^T += V^T P^T with mma.sync m16n8k16: keys,
 // then head columns, in the 16 rows, the query rows in the 8 columns, so that 8 of them fill an instruction.  Operands come straight
 // from global memory, 16 bytes per lane and load: the contraction runs over the head columns in the order in which the lanes hold
@@ -63,7 +80,7 @@ __device__ __forceinline__ float weight_of(float m, float most) { return exp2f(m
 // products; a warp has 8 KB (heads of 128) in flight.  Rows past the run's end are not read: their registers are zero.
 // Lane (g, t4) = (lane / 4, lane % 4).
 template <typename T, int D, int NT> struct KeyWalk {
-    static constexpr int KC = D / 32, VC = D / 64, R = 8 * NT;
+    static constexpr int KC = D / 32, VC = D / 64;
     uint4 qf[NT][KC];                                     // row n * 8 + g, columns 32 c + 8 t4 ..
     uint4 kf[2][KC], vf[4][VC];                           // keys g, g + 8, the same columns; keys 2 t4, + 1, + 8, + 9, columns 64 c + 8 g ..
     float o[NT][D / 16][4];                               // tile (c, i): columns d = 64 c + 8 g + 2 i and + 1 of rows n * 8 + 2 t4 and + 1
@@ -180,8 +197,9 @@ template <typename T, int D, int NT> struct KeyWalk {
     }
 };
 
-// The sequences' own keys (and the prefix's where it has no launch of its own), and the merge.  One cluster of `gridDim.x` CTAs per
-// (sequence, key head, 8 * NT query rows); a warp takes every (warps of the cluster)-th block of 16 keys.
+// The sequences' own keys, and the prefix's where it has no launch of its own.  `gridDim.x` CTAs per unit, which is (sequence, key head, 8 * NT
+// query rows); a warp takes every (warps of the unit)-th block of 16 keys.  With the prefix apart the CTAs leave parts for
+// merge_kernel; else they are a cluster and merge through distributed shared memory.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kOwnThreads, NT == 1 ? 4 : D == 64 ? 3 : 2)
 own_kernel(const OwnParams p) {
@@ -189,7 +207,8 @@ own_kernel(const OwnParams p) {
     __shared__ __align__(16) float s_o[kOwnWarps][R][D + 4];
     __shared__ float s_ml[kOwnWarps][R][2];
     __shared__ float s_sum_ml[R][2];                      // the CTA's, for the cluster; its O takes the first warp's place
-    __shared__ float s_w[R][kMostOwnCluster + kMostSplits];
+    __shared__ float s_w[R][kMostOwnCluster];
+    griddep_launch_dependents();                          // the merge may get ready
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int ctas = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y / p.row_groups, r0 = (blockIdx.y % p.row_groups) * R, b = blockIdx.z;
     const int rows = min(R, p.group - r0), nQH = p.nKVH * p.group, head0 = kvh * p.group + r0;
@@ -218,6 +237,29 @@ own_kernel(const OwnParams p) {
     }
     w.result([&](int row, float m, float l) { s_ml[warp][row][0] = m; s_ml[warp][row][1] = l; }, [&](int row, int d, float4 v) { *reinterpret_cast<float4*>(&s_o[warp][row][d]) = v; });
     __syncthreads();
+    if (p.apart) {                                        // the CTA's result is a part
+        const size_t row0 = (size_t(p.first_part + rank) * p.batch + b) * nQH + head0;
+        for (int i = threadIdx.x; i < rows * (D / 4); i += kOwnThreads) {
+            const int row = i / (D / 4), d = i % (D / 4) * 4;
+            float most = -INFINITY, sum = 0.f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            #pragma unroll
+            for (int k = 0; k < kOwnWarps; ++k) most = fmaxf(most, s_ml[k][row][0]);
+            #pragma unroll
+            for (int k = 0; k < kOwnWarps; ++k) {
+                const float f = weight_of(s_ml[k][row][0], most);
+                const float4 v = *reinterpret_cast<const float4*>(&s_o[k][row][d]);
+                sum += f * s_ml[k][row][1];
+                x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
+            }
+            *reinterpret_cast<float4*>(&p.part_o[(row0 + row) * D + d]) = x;
+            if (d == 0) *reinterpret_cast<float2*>(&p.part_ml[2 * (row0 + row)]) = make_float2(most, sum);
+        }
+        // One CTA's wait for the prefix's launch is this launch's: the merge waits for this one alone.  (All CTAs': those that are done
+        // held the SMs that others could have begun on.)
+        if (blockIdx.x + blockIdx.y + blockIdx.z == 0) griddep_wait();
+        return;
+    }
     // the CTA's, where a cluster follows
     if (ctas > 1) {
         for (int i = threadIdx.x; i < rows * D; i += kOwnThreads) {
@@ -231,38 +273,16 @@ own_kernel(const OwnParams p) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    griddep_wait();                                       // the prefix's splits are there
-    // every part's weight in the sum, 2^(m_i - m) / l, a warp per row: the warps (or the cluster's CTAs), then the prefix's splits
+    // every part's weight in the sum, 2^(m_i - m) / l: a warp per row
     const int parts = ctas > 1 ? ctas : kOwnWarps;
-    const size_t part0 = size_t(b) * nQH + head0, next = size_t(p.batch) * nQH;
     for (int row = warp; row < rows; row += kOwnWarps) {
-        float2 ml[kMostSplits / 32 + 1];                  // lane i: part i, then the splits i, 32 + i, ...
-        ml[0] = make_float2(-INFINITY, 0.f);
+        float2 ml = make_float2(-INFINITY, 0.f);
         if (lane < parts)
-            ml[0] = ctas > 1 ? make_float2(load_cluster_f32(dme::smem_addr(&s_sum_ml[row][0]), lane), load_cluster_f32(dme::smem_addr(&s_sum_ml[row][1]), lane))
-                             : make_float2(s_ml[lane][row][0], s_ml[lane][row][1]);
-        float most = ml[0].x;
-        #pragma unroll
-        for (int k = 0; k < kMostSplits / 32; ++k) {
-            const int s = 32 * k + lane;
-            ml[k + 1] = s < p.splits ? *reinterpret_cast<const float2*>(&p.part_ml[2 * (part0 + row + s * next)]) : make_float2(-INFINITY, 0.f);
-            most = fmaxf(most, ml[k + 1].x);
-        }
-        #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        float sum = 0.f;
-        #pragma unroll
-        for (int k = 0; k <= kMostSplits / 32; ++k) {
-            const float f = ml[k].y == 0.f ? 0.f : weight_of(ml[k].x, most);        // a sum of 0: no key
-            sum += f * ml[k].y;
-            ml[k].x = f;
-        }
-        #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float inv = p.prefix_len + own > 0 ? 1.f / sum : 0.f;
-        if (lane < parts) s_w[row][lane] = ml[0].x * inv;
-        #pragma unroll
-        for (int k = 0; k < kMostSplits / 32; ++k) if (32 * k + lane < p.splits) s_w[row][kMostOwnCluster + 32 * k + lane] = ml[k + 1].x * inv;
+            ml = ctas > 1 ? make_float2(load_cluster_f32(dme::smem_addr(&s_sum_ml[row][0]), lane), load_cluster_f32(dme::smem_addr(&s_sum_ml[row][1]), lane))
+                          : make_float2(s_ml[lane][row][0], s_ml[lane][row][1]);
+        float inv;
+        const float f = part_weight(ml, inv);
+        if (lane < parts) s_w[row][lane] = p.prefix_here + own > 0 ? f * inv : 0.f;
     }
     __syncthreads();
     // four columns per thread
@@ -270,17 +290,10 @@ own_kernel(const OwnParams p) {
     for (int i = rank * share + threadIdx.x; i < last; i += kOwnThreads) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
         float x[4] = {0.f, 0.f, 0.f, 0.f};
-        auto add = [&](float f, const float4& v) { x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w; };
-        const float* o_part = p.part_o + (part0 + row) * D + d;
-        #pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) {
-            const float f = s_w[row][kMostOwnCluster + s];
-            const float4 v = *reinterpret_cast<const float4*>(o_part + s * next * D);
-            if (f != 0.f) add(f, v);                      // where a split had no key for the row nothing was stored
-        }
         for (int k = 0; k < parts; ++k) {
             const float4 v = ctas > 1 ? load_cluster_f32x4(dme::smem_addr(&s_o[0][row][d]), k) : *reinterpret_cast<const float4*>(&s_o[k][row][d]);
-            add(s_w[row][k], v);
+            const float f = s_w[row][k];
+            x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
         }
         T* y = static_cast<T*>(p.o) + b * p.o_batch + (long long)(head0 + row) * D + d;
         *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
@@ -291,49 +304,125 @@ own_kernel(const OwnParams p) {
     }
 }
 
+// The parts of a row (the prefix's splits, the CTAs of the sequence's own keys) into its result: a warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(kOwnThreads)
+merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int parts, int rows, int nQH, T* __restrict__ o, long long o_batch) {
+    constexpr int E = D / 32;
+    __shared__ float s_f[kOwnWarps][kMostParts];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x * kOwnWarps + warp;
+    griddep_wait();
+    if (row >= rows) return;
+    float2 ml[kMostParts / 32];
+    float most = -INFINITY;
+    #pragma unroll
+    for (int k = 0; k < kMostParts / 32; ++k) {
+        const int s = 32 * k + lane;
+        ml[k] = s < parts ? __ldcg(reinterpret_cast<const float2*>(&part_ml[2 * (size_t(s) * rows + row)])) : make_float2(-INFINITY, 0.f);
+        most = fmaxf(most, ml[k].x);
+    }
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    float sum = 0.f;
+    #pragma unroll
+    for (int k = 0; k < kMostParts / 32; ++k) {
+        const float f = ml[k].y == 0.f ? 0.f : weight_of(ml[k].x, most);
+        sum += f * ml[k].y;
+        if (32 * k + lane < kMostParts) s_f[warp][32 * k + lane] = f;
+    }
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    __syncwarp();
+    float x[E] = {};
+    #pragma unroll 8
+    for (int s = 0; s < parts; ++s) {
+        float v[E];
+        const float* at = part_o + (size_t(s) * rows + row) * D + lane * E;
+        if constexpr (E == 4) { const float4 w = __ldcg(reinterpret_cast<const float4*>(at)); v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w; }
+        else { const float2 w = __ldcg(reinterpret_cast<const float2*>(at)); v[0] = w.x; v[1] = w.y; }
+        const float f = s_f[warp][s];
+        #pragma unroll
+        for (int e = 0; e < E; ++e) if (f != 0.f) x[e] += f * v[e];
+    }
+    const float inv = 1.f / sum;
+    T* y = o + row / nQH * o_batch + (long long)(row % nQH) * D + lane * E;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
+    else *reinterpret_cast<uint32_t*>(y) = pack2<T>(x[0] * inv, x[1] * inv);
+}
+
 // How a call is run.
-enum PrefixKind { PREFIX_NONE, PREFIX_HERE, PREFIX_TILES };       // no keys; by own_kernel, per sequence; a launch of the tcgen05 kernel
 struct SharedPlan {
-    int prefix;
-    int splits, span;            // PREFIX_TILES: of its launch; span: tiles of an item
-    int cluster, rows;           // CTAs and query rows (8 or 16) of a unit of the second launch
+    int splits, span;            // the prefix in a launch of its own: its splits, tiles of an item; 0: none, own_kernel reads the prefix
+    int cluster, rows;           // CTAs and query rows (8 or 16) of a unit of own_kernel
     size_t off_ml, ws_bytes;
 };
 
+// Times in microseconds, from sizes alone, as they were measured over the range (sequences 2 to 256, prefixes of 100 to 32768 keys, 1 to 8
+// key heads of 64 and 128, own caches up to 2000; a choice is within 15 % of the best one tried).  The sequences' own lengths are not known
+// here: a little over half the caches' room.
+//  * own_kernel alone: 4.5, and what it reads (the prefix for every sequence, from L2) at 7 TB/s or a warp's blocks of 16 keys at 0.6 each.
+//    (32 / 8 heads of 128, 4 sequences, 512 keys in front: 6.2 against 8.0 with the prefix apart; 32 sequences, 2000 keys: 41 against 17.)
+//  * the prefix apart: 5.5 for the launches and the merge; an item of the tcgen05 kernel takes 4.5 and 1.35 per key tile, 2.05 with two
+//    query tiles; the own keys are read at 44 GB/s per SM, by the SMs that have no item and, once the items are done, by all; the parts are
+//    written and read again.  (32 sequences, 2000 + up to 512 keys: 4 splits on 32 SMs 16.9, 8 on 64 18.9, 2 on 16 22.6.)
 SharedPlan plan_shared(const b200p_shared_args& a) {
     SharedPlan pl{};
     const int sms = sm_count() > 0 ? sm_count() : 148, group = a.nQHeads / a.nKVHeads;
     pl.rows = group <= 8 ? 8 : 16;
     const long long units = (long long)a.batch * a.nKVHeads * ((group + pl.rows - 1) / pl.rows);
-    if (a.prefix_len == 0) pl.prefix = PREFIX_NONE;
-    else if ((long long)a.batch * a.prefix_len <= 4096) pl.prefix = PREFIX_HERE;
-    else pl.prefix = PREFIX_TILES;
-    const int forced = tuning(KNOB_SHARED_PREFIX, 0);
-    if (a.prefix_len > 0 && forced >= PREFIX_HERE && forced <= PREFIX_TILES) pl.prefix = forced;
-    if (pl.prefix == PREFIX_TILES) {
-        const int tokens = kBM / group, tiles = (a.batch + tokens - 1) / tokens, steps = (a.prefix_len + kBN - 1) / kBN;
-        double best = 0;
-        const int forced_splits = tuning(KNOB_SHARED_SPLITS, 0);
-        for (int s = 1; s <= steps && s <= kMostSplits; ++s) {
-            if (forced_splits > 0 && s != (forced_splits < steps ? forced_splits : steps)) continue;
-            for (int span = 1; span <= 2; ++span) {
-                if (span == 2 && tiles == 1) continue;
-                const long long items = (long long)(tiles + span - 1) / span * a.nKVHeads * s;
-                const double step = span == 1 ? 1.0 : 1.7;                    // in steps of one tile, 1.2 us
-                const double t = double((items + sms - 1) / sms) * ((steps + s - 1) / s * step + 2.0) + double(s) * a.batch * a.nQHeads * a.D * 8 / 7.8e6;
-                if (best == 0 || t < best) { best = t; pl.splits = s; pl.span = span; }
-            }
+    auto cluster_for = [&](long long keys) {                    // CTAs of a unit: as many as find work and room
+        int c = 1;
+        while (c < kMostOwnCluster && units * c < 2 * sms && keys > 2 * kKeyBlock * kOwnWarps * c) c *= 2;
+        return c;
+    };
+    pl.cluster = cluster_for((long long)a.max_own + a.prefix_len);
+    if (a.prefix_len == 0) return pl;
+    const double own_keys = 0.55 * a.max_own, key_bytes = 4.0 * a.D * a.nKVHeads;
+    const double here_bytes = a.batch * (a.prefix_len + own_keys) * key_bytes;
+    const double here_walk = 0.6 * ((a.prefix_len + own_keys) / (kKeyBlock * kOwnWarps * pl.cluster) + 1);
+    const double here = 4.5 + (here_bytes / 7e6 > here_walk ? here_bytes / 7e6 : here_walk);
+    const double own_work = a.batch * own_keys * key_bytes / 44e3;              // of one SM
+    const int tokens = kBM / group, tiles = (a.batch + tokens - 1) / tokens, steps = (a.prefix_len + kBN - 1) / kBN, fixed = tuning(KNOB_SHARED_SPLITS, 0);
+    double best = 0;
+    int splits = 0, span = 0;
+    for (int per = 1; per <= steps; ++per) {                    // key tiles of an item
+        const int s = (steps + per - 1) / per;
+        if (s > kMostSplits || (per > 1 && s == (steps + per - 2) / (per - 1) && fixed == 0)) continue;
+        if (fixed > 0 && per != (steps + fixed - 1) / fixed) continue;
+        for (int sp = 1; sp <= (tiles > 1 ? 2 : 1); ++sp) {
+            const long long items = (long long)(tiles + sp - 1) / sp * a.nKVHeads * s;
+            const double item = 4.5 + per * (sp == 1 ? 1.35 : 2.05), parts = double(s) * a.batch * a.nQHeads * a.D * 8 / 7.8e6;
+            double t;
+            if (items < sms) {
+                const double alone = own_work / double(sms - items);            // the own keys on the SMs without an item
+                t = alone + 2 <= item ? item : item + (alone + 2 - item) / alone * own_work / sms + 4;
+            } else t = double((items + sms - 1) / sms) * item + own_work / sms + 5;
+            if (best == 0 || t + parts < best) { best = t + parts; splits = s; span = sp; }
         }
     }
-    if (pl.splits > 0) {
-        const size_t all = size_t(pl.splits) * a.batch * a.nQHeads;
+    const int forced = tuning(KNOB_SHARED_PREFIX, 0);
+    if (splits > 0 && forced != 1 && (forced == 2 || 5.5 + best < here)) {
+        pl.splits = splits; pl.span = span;
+        pl.cluster = cluster_for(a.max_own);
+        const size_t all = size_t(pl.splits + pl.cluster) * a.batch * a.nQHeads;
         pl.off_ml = (all * a.D * 4 + 255) / 256 * 256;
         pl.ws_bytes = pl.off_ml + (all * 8 + 255) / 256 * 256;
     }
-    const long long keys = a.max_own + (pl.prefix == PREFIX_HERE ? a.prefix_len : 0);
-    pl.cluster = 1;
-    while (pl.cluster < kMostOwnCluster && units * pl.cluster < 2 * sms && keys > 2 * kKeyBlock * kOwnWarps * pl.cluster) pl.cluster *= 2;
     return pl;
+}
+
+// A launch that may get ready while the stream's last one runs (it calls griddep_wait for its results).
+template <typename... P, typename... A>
+int launch_after(void (*kern)(P...), dim3 grid, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(kOwnThreads); cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) { cudaGetLastError(); return int(e); }
+    return launched();
 }
 
 template <typename T, int D, int NT>
@@ -342,7 +431,7 @@ int launch_own(const OwnParams& p, int cluster, bool dependent, cudaStream_t st)
     cfg.gridDim = dim3(unsigned(cluster), unsigned(p.nKVH * p.row_groups), unsigned(p.batch)); cfg.blockDim = dim3(kOwnThreads); cfg.stream = st;
     cudaLaunchAttribute attr[2];
     int n = 0;
-    if (cluster > 1) {
+    if (cluster > 1 && !p.apart) {
         attr[n].id = cudaLaunchAttributeClusterDimension;
         attr[n].val.clusterDim.x = unsigned(cluster); attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
         ++n;
@@ -365,7 +454,8 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
     const int group = a.nQHeads / a.nKVHeads;
     float* part_o = static_cast<float*>(workspace);
     float* part_ml = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pl.off_ml);
-    if (pl.prefix == PREFIX_TILES) {
+    const bool apart = pl.splits > 0;
+    if (apart) {
         PackedParams p{};
         p.Q = q; p.K = Kp; p.V = Vp;
         p.seqQ = a.batch; p.seqK = a.prefix_len; p.batch = 1;
@@ -375,14 +465,17 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
         p.part_o = part_o; p.part_ml = part_ml;
         if (int e = launch_packed<T, D, true>(p, a.dtype, st)) return e;
     }
-    const bool apart = pl.splits > 0;
     OwnParams w{};
     w.q = q; w.Kp = Kp; w.Vp = Vp; w.K = K; w.V = V; w.o = o; w.lengths = lengths;
     w.batch = a.batch; w.nKVH = a.nKVHeads; w.group = group; w.max_own = a.max_own; w.row_groups = (group + pl.rows - 1) / pl.rows;
-    w.prefix_here = pl.prefix == PREFIX_HERE ? a.prefix_len : 0; w.prefix_len = a.prefix_len;
+    w.prefix_here = apart ? 0 : a.prefix_len;
     w.prefix_head = a.prefix_head; w.own_head = a.own_head; w.own_batch = a.own_batch; w.q_batch = a.q_batch; w.o_batch = a.o_batch;
-    w.scale_log2 = scale_log2; w.splits = pl.splits; w.part_o = part_o; w.part_ml = part_ml;
-    return pl.rows == 8 ? launch_own<T, D, 1>(w, pl.cluster, apart, st) : launch_own<T, D, 2>(w, pl.cluster, apart, st);
+    w.scale_log2 = scale_log2; w.apart = apart; w.first_part = pl.splits; w.part_o = part_o; w.part_ml = part_ml;
+    if (int e = pl.rows == 8 ? launch_own<T, D, 1>(w, pl.cluster, apart, st) : launch_own<T, D, 2>(w, pl.cluster, apart, st)) return e;
+    if (!apart) return B200P_OK;
+    const int rows = a.batch * a.nQHeads;
+    return launch_after(merge_kernel<T, D>, dim3(unsigned((rows + kOwnWarps - 1) / kOwnWarps)), st, static_cast<const float*>(part_o), static_cast<const float*>(part_ml),
+                        pl.splits + pl.cluster, rows, a.nQHeads, static_cast<T*>(o), a.o_batch);
 }
 
 int checked(const b200p_shared_args* args, b200p_shared_args* out) {
@@ -392,7 +485,7 @@ int checked(const b200p_shared_args* args, b200p_shared_args* out) {
     if (a.D != 64 && a.D != 128) return B200P_E_DIM;
     if (a.nQHeads <= 0 || a.nKVHeads <= 0 || a.nQHeads % a.nKVHeads != 0) return B200P_E_DIM;
     if (a.batch < 0 || a.prefix_len < 0 || a.max_own < 0 || !(a.scale >= 0.f) || std::isinf(a.scale)) return B200P_E_LENGTH;
-    if (a.nQHeads / a.nKVHeads > 128 || a.nQHeads > 65535 || a.batch > 65535) return B200P_E_RANGE;
+    if (a.nQHeads / a.nKVHeads > 128 || a.nQHeads > 65535 || a.batch > 65535 || (long long)a.batch * a.nQHeads > (1 << 28)) return B200P_E_RANGE;
     const long long D = a.D;
     if (a.prefix_head == 0) a.prefix_head = a.prefix_len * D;
     if (a.own_head == 0) a.own_head = a.max_own * D;
