@@ -62,6 +62,7 @@ SYMBOLS = {
     "b200p_session_create": (_vp, [_vp, _i, _i, _vp]),
     "b200p_session_open": (_vp, [_vp, _i, _i, _i, _vp]),
     "b200p_session_extend": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp]),
+    "b200p_session_set_rules": (_i, [_vp, _vp]),
     "b200p_session_reset": (None, [_vp]),
     "b200p_session_destroy": (None, [_vp]),
     "b200p_session_generate": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp]),
@@ -848,6 +849,11 @@ def gemm_16(A, W, out, epilogue: str = "store16"):
     return out
 
 
+class SessionRules(C.Structure):
+    """struct b200p_session_rules (include/b200p_runtime.h)."""
+    _fields_ = [("repetition", C.c_float), ("presence", C.c_float), ("frequency", C.c_float), ("bias_n", _i), ("bias_ids", _vp), ("bias_values", _vp), ("mask", _vp)]
+
+
 class Session:
     """Greedy-decoding session over caller-owned weights.
 
@@ -919,6 +925,29 @@ class Session:
         _check(lib().b200p_session_generate(self._h, a.ctypes.data, a.shape[1], max_new_tokens, out.ctypes.data, tm,
                                             self._stream()), "session_generate")
         return out, (tm[0], tm[1])
+
+    def set_rules(self, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias=None, allowed=None, banned=None):
+        """Rules on generate()'s logits, for all sequences, as adjust_logits has them: penalties for tokens of the prompt and of
+        the answer so far, bias {token: value}, allowed tokens (all others are never picked) and banned ones.  Without arguments the
+        rules are taken back.  The other calls return logits without rules."""
+        import numpy as np
+        bias = dict(bias or {})
+        V = self.cfg["vocab_size"]
+        mask = None
+        if allowed is not None or banned is not None:
+            keep = np.ones((V + 31) // 32 * 32, np.uint8) if allowed is None else np.zeros((V + 31) // 32 * 32, np.uint8)
+            for tokens, bit in ((allowed, 1), (banned, 0)):
+                tokens = np.asarray([] if tokens is None else list(tokens), np.int64)
+                if len(tokens) and (tokens.min() < 0 or tokens.max() >= V):
+                    raise ValueError("allowed and banned tokens must be in the vocabulary")
+                keep[tokens] = bit
+            mask = np.packbits(keep, bitorder="little").view(np.uint32)
+        if not bias and mask is None and (repetition, presence, frequency) == (1.0, 0.0, 0.0):
+            _check(lib().b200p_session_set_rules(self._h, None), "session_set_rules")
+            return
+        ids, values = np.asarray(list(bias), np.int32), np.asarray(list(bias.values()), np.float32)
+        r = SessionRules(repetition, presence, frequency, len(ids), ids.ctypes.data, values.ctypes.data, mask.ctypes.data if mask is not None else None)
+        _check(lib().b200p_session_set_rules(self._h, C.byref(r)), "session_set_rules")
 
     def prefill_logits(self, input_ids):
         import numpy as np

@@ -15,7 +15,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kSegment = 32 * kThreads;          // tokens a CTA handles, a word of shared memory for each
-constexpr int kMostBias = 1024;
 // A token's word: how often it was generated, and two flags.
 constexpr unsigned kInPrompt = 1u << 31, kBiased = 1u << 30, kCount = kBiased - 1;
 

@@ -19,7 +19,9 @@
 #include "session.cuh"
 #include "model.hpp"
 #include "status_rc.hpp"
+#include "logits.cuh"
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace b200p {
@@ -300,6 +302,16 @@ int embed(b200p_session* s, const int* ids, int M, cudaStream_t st) {
 // argmax: rows x slices of ~2048 logits
 int sample(b200p_session* s, int max_new, int step, const int* step_dev, cudaStream_t st) {
     const int V = s->c.vocab_size;
+    if (s->rules.on) {                                          // in place; *step_dev tokens of a row are generated so far, 0 after the prompt
+        b200p_logits_args a{};
+        a.dtype = B200P_F32; a.rows = s->batch; a.vocab = V; a.in_stride = a.out_stride = V;
+        a.prompt = s->d_ids; a.prompt_max = s->prompt_len;
+        if (step_dev) { a.tokens = s->d_tokens; a.tokens_max = max_new; a.token_lengths = step_dev; }
+        a.repetition = s->rules.repetition; a.presence = s->rules.presence; a.frequency = s->rules.frequency;
+        a.bias_ids = s->rules.bias_ids; a.bias_values = s->rules.bias_values; a.bias_n = s->rules.bias_n;
+        if (s->rules.masked) { a.mask = s->rules.mask; a.mask_rows = s->rules.mask_rows; a.n_masks = 1; }
+        if (int e = logits_adjust(s->logits, s->logits, &a, 0, 0, st)) return e;
+    }
     return with_type(s->dtype, [&](auto tag) -> int {
         using T = decltype(tag);
         argmax_kernel<T><<<dim3(unsigned(s->batch), unsigned((V + 2047) / 2048)), 256, 0, st>>>(
@@ -348,6 +360,7 @@ int build_step_graph(b200p_session* s, int max_new) {
     cudaGraphDestroy(graph);
     if (ie != cudaSuccess) { s->step_graph = nullptr; cudaGetLastError(); return int(ie); }
     s->graph_hidden = s->hidden; s->graph_tokens = s->d_tokens; s->graph_max_new = max_new; s->graph_epoch = tuning_epoch();
+    s->graph_prompt = s->prompt_len;
     return B200P_OK;
 }
 
@@ -374,6 +387,7 @@ int generate(b200p_session* s, const int* ids, int Tn, int max_new, int* out, fl
         if ((rc = clear_status(s, st))) break;
         cudaEventRecord(e0, st);
         if (cudaError_t e = cudaMemcpyAsync(s->d_ids, ids, size_t(B) * Tn * sizeof(int), cudaMemcpyHostToDevice, st)) { rc = int(e); break; }
+        s->prompt_len = Tn;
         if ((rc = embed(s, s->d_ids, B * Tn, st))) break;
         s->kv_len = 0;
         if ((rc = s->ops->run_layers(s, Tn, 0, st, nullptr))) break;
@@ -384,7 +398,7 @@ int generate(b200p_session* s, const int* ids, int Tn, int max_new, int* out, fl
         if ((rc = launched())) break;
         cudaEventRecord(e1, st);
         bool looped = false;
-        if (max_new > 1 && s->ops->decode_loop) {
+        if (max_new > 1 && s->ops->decode_loop && !s->rules.on) {
             // all remaining steps in one launch: the ids, the position and the output column stay on the device
             if (Tn + max_new - 2 >= s->max_seq) { rc = B200P_E_RANGE; break; }
             if ((rc = s->ops->decode_loop(s, s->d_next, max_new - 1, true, s->d_tokens, max_new, st, &looped))) break;
@@ -395,7 +409,7 @@ int generate(b200p_session* s, const int* ids, int Tn, int max_new, int* out, fl
             if (use_graph && step >= 2) {
                 // the first decode step ran eagerly below; from the second on, replay the captured step
                 if (!s->step_graph || s->graph_hidden != s->hidden || s->graph_tokens != s->d_tokens || s->graph_max_new != max_new ||
-                    s->graph_epoch != tuning_epoch()) {
+                    s->graph_epoch != tuning_epoch() || (s->rules.on && s->graph_prompt != s->prompt_len)) {
                     if (build_step_graph(s, max_new) != B200P_OK) drop_step_graph(s);
                 }
                 if (s->step_graph) {
@@ -591,6 +605,43 @@ extern "C" int b200p_session_extend(b200p_session* s, const int* ids, int T, con
     for (int i = 0; i < n_want; ++i) if (want[i] < 0 || want[i] >= T) return B200P_E_RANGE;
     if (!ids_exist(s, ids, size_t(s->batch) * T)) return B200P_E_RANGE;
     return extend(s, ids, T, want, n_want, logits, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200p_session_set_rules(b200p_session* s, const b200p_session_rules* r) {
+    if (!s) return B200P_E_NULL;
+    if (!r) {
+        if (s->rules.on) drop_step_graph(s);
+        s->rules.on = false;
+        return B200P_OK;
+    }
+    if (!(r->repetition > 0.f) || std::isinf(r->repetition) || !std::isfinite(r->presence) || !std::isfinite(r->frequency)) return B200P_E_RANGE;
+    if (r->bias_n < 0) return B200P_E_LENGTH;
+    if (r->bias_n > kMostBias) return B200P_E_RANGE;
+    if (r->bias_n > 0 && (!r->bias_ids || !r->bias_values)) return B200P_E_NULL;
+    if (!ids_exist(s, r->bias_ids, size_t(r->bias_n))) return B200P_E_RANGE;
+    for (int i = 0; i < r->bias_n; ++i) if (std::isnan(r->bias_values[i])) return B200P_E_RANGE;
+    const size_t B = size_t(s->batch), words = (size_t(s->c.vocab_size) + 31) / 32;
+    auto& d = s->rules;
+    if (!d.mask) {
+        cudaError_t e;
+        if ((e = s->alloc(&d.repetition, B * 4)) || (e = s->alloc(&d.presence, B * 4)) || (e = s->alloc(&d.frequency, B * 4)) || (e = s->alloc(&d.mask_rows, B * 4)) ||
+            (e = s->alloc(&d.bias_ids, B * kMostBias * 4)) || (e = s->alloc(&d.bias_values, B * kMostBias * 4)) || (e = cudaMemset(d.mask_rows, 0, B * 4)) ||
+            (e = s->alloc(&d.mask, words * 4))) return int(e);                       // the last: its pointer says that all are there
+    }
+    d.on = false;
+    drop_step_graph(s);
+    const std::vector<float> rep(B, r->repetition), pres(B, r->presence), freq(B, r->frequency);
+    std::vector<int> ids; std::vector<float> values;
+    for (size_t b = 0; b < B; ++b) { ids.insert(ids.end(), r->bias_ids, r->bias_ids + r->bias_n); values.insert(values.end(), r->bias_values, r->bias_values + r->bias_n); }
+    cudaError_t e;
+    if ((e = cudaMemcpy(d.repetition, rep.data(), B * 4, cudaMemcpyHostToDevice)) || (e = cudaMemcpy(d.presence, pres.data(), B * 4, cudaMemcpyHostToDevice)) ||
+        (e = cudaMemcpy(d.frequency, freq.data(), B * 4, cudaMemcpyHostToDevice)) ||
+        (!ids.empty() && ((e = cudaMemcpy(d.bias_ids, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice)) ||
+                          (e = cudaMemcpy(d.bias_values, values.data(), values.size() * 4, cudaMemcpyHostToDevice)))) ||
+        (r->mask && (e = cudaMemcpy(d.mask, r->mask, words * 4, cudaMemcpyHostToDevice)))) return int(e);
+    d.bias_n = r->bias_n; d.masked = r->mask != nullptr;
+    d.on = true;
+    return B200P_OK;
 }
 
 extern "C" void b200p_session_reset(b200p_session* s) { if (s) s->kv_len = 0; }

@@ -130,6 +130,15 @@ struct b200p_session {
     unsigned long long graph_replays = 0, graph_kernels = 0;   // kernels of this library inside one replay
     unsigned long long gemm_calls = 0, blas_calls = 0;      // all projections / those that went to the GEMM library
     unsigned long long mega_launches = 0;
+    // rules on the greedy loop's logits (b200p_session_set_rules), the same for every sequence; one copy per row for the kernel
+    struct {
+        bool on = false, masked = false;
+        int bias_n = 0;
+        float *repetition = nullptr, *presence = nullptr, *frequency = nullptr, *bias_values = nullptr;
+        int *bias_ids = nullptr, *mask_rows = nullptr;
+        unsigned* mask = nullptr;
+    } rules;
+    int prompt_len = 0, graph_prompt = 0;                // tokens of the prompt in d_ids; those that the captured step counts
     std::vector<void*> owned, scratch;                   // for the session's life / for the current cap_tokens
 
     template <typename P> cudaError_t alloc(P** p, size_t bytes) { return alloc_in(owned, p, bytes); }

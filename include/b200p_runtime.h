@@ -105,6 +105,22 @@ b200p_session* b200p_session_open(const b200p_model* model, int dtype, int max_s
 int b200p_session_generate(b200p_session* s, const int* input_ids, int T, int max_new_tokens,
                            int* out_tokens, float* timings_ms, b200p_stream_t stream);
 
+/* Rules on the logits of b200p_session_generate, the same for every sequence (b200p_logits_adjust, b200p.h, says
+ * what each does): from the next call on the token picked is the largest adjusted logit, with the call's prompt
+ * and the tokens generated in the call as the history.  bias_ids and bias_values: host, bias_n entries (at most
+ * 1024); mask: host, (vocab + 31) / 32 words, token t in bit t % 32 of word t / 32, or NULL.  rules = NULL takes them
+ * back.  The other calls return logits without rules.  B200P_E_RANGE for a repetition that is not positive, values
+ * that are no numbers, ids that do not exist. */
+typedef struct b200p_session_rules {
+    float repetition;          /* 1: none */
+    float presence, frequency; /* 0: none */
+    int bias_n;
+    const int* bias_ids;
+    const float* bias_values;
+    const unsigned* mask;
+} b200p_session_rules;
+int b200p_session_set_rules(b200p_session* s, const b200p_session_rules* rules);
+
 /* Session::prefill_logits (session.hpp:299-318): prefill only; fp32 logits of the
  * last prompt token of every sequence, host [batch, vocab]. */
 int b200p_session_prefill_logits(b200p_session* s, const int* input_ids, int T, float* logits, b200p_stream_t stream);

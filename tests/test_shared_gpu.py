@@ -33,6 +33,22 @@ def test_prefix_and_own_keys(b200p, torch_cuda, batch, heads, kv, prefix, own, D
     close(got, *ref.shared(*x, n, prefix))
 
 
+# every way to run a call, whatever the sizes would choose: the prefix per sequence, or once, in few and in many splits
+@pytest.mark.parametrize("form,splits", [(1, -1), (2, -1), (2, 1), (2, 3), (2, 1000)])
+@pytest.mark.parametrize("batch,heads,kv,D,prefix,own", [(1, 4, 4, 128, 1, 5), (3, 6, 2, 64, 257, 40), (40, 8, 1, 128, 1000, 200), (9, 40, 8, 64, 700, 33), (150, 4, 2, 128, 300, 100),
+                                                         (2, 20, 1, 128, 513, 600)])
+def test_every_form(b200p, torch_cuda, batch, heads, kv, D, prefix, own, form, splits):
+    torch = torch_cuda
+    x = make(torch, batch, heads, kv, D, prefix, own, torch.bfloat16, seed=batch)
+    n = spread(batch, own)
+    try:
+        b200p.set_tuning("shared_prefix", form), b200p.set_tuning("shared_splits", splits)
+        got = b200p.decode_shared(*x, torch.tensor(n, dtype=torch.int32, device="cuda"))
+    finally:
+        b200p.set_tuning("shared_prefix", -1), b200p.set_tuning("shared_splits", -1)
+    close(got, *ref.shared(*x, n, prefix))
+
+
 # long caches of few sequences, long prefixes, both
 @pytest.mark.parametrize("batch,heads,kv,D,prefix,own", [(1, 8, 1, 128, 9000, 5000), (2, 8, 2, 64, 300, 9001), (2, 4, 4, 128, 20000, 10), (64, 8, 2, 128, 4096, 500)])
 def test_long(b200p, torch_cuda, batch, heads, kv, D, prefix, own):
