@@ -385,10 +385,10 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
     const int tokens = kBM / group, tiles = (a.batch + tokens - 1) / tokens, steps = (a.prefix_len + kBN - 1) / kBN, fixed = tuning(KNOB_SHARED_SPLITS, 0);
     double best = 0;
     int splits = 0, span = 0;
-    for (int per = 1; per <= steps; ++per) {                    // key tiles of an item
+    const int first = fixed > 0 ? fixed : kMostSplits;
+    for (int per = (steps + first - 1) / first, next; per > 0; per = next) {    // key tiles of an item; the next is the smallest with fewer splits
         const int s = (steps + per - 1) / per;
-        if (s > kMostSplits || (per > 1 && s == (steps + per - 2) / (per - 1) && fixed == 0)) continue;
-        if (fixed > 0 && per != (steps + fixed - 1) / fixed) continue;
+        next = s > 1 && fixed == 0 ? (steps + s - 2) / (s - 1) : 0;
         for (int sp = 1; sp <= (tiles > 1 ? 2 : 1); ++sp) {
             const long long items = (long long)(tiles + sp - 1) / sp * a.nKVHeads * s;
             const double item = 4.5 + per * (sp == 1 ? 1.35 : 2.05), parts = double(s) * a.batch * a.nQHeads * a.D * 8 / 7.8e6;

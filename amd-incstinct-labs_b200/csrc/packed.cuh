@@ -96,7 +96,8 @@ __device__ __forceinline__ bool packed_walk(const PackedParams& p, void* answer,
         return there ? __shfl_sync(kAll, x, 0) : -2;
     };
     int most = 0, blocks = 0, chunk_most = 0;                   // key tiles of the longest sequence, blocks of all; lane c: of chunk c
-    for (int c = 0; c < chunks; ++c) {
+    #pragma unroll 4
+    for (int c = 0; c < chunks; ++c) {                          // (four loads under way)
         load(c);
         blocks += (n + block - 1) / block;
         const int tiles = __reduce_max_sync(kAll, n == 0 ? 0 : max(1, (m + kBN - 1) / kBN));

@@ -22,6 +22,7 @@
 #include "logits.cuh"
 #include <algorithm>
 #include <cmath>
+#include <new>
 #include <type_traits>
 
 namespace b200p {
@@ -607,7 +608,7 @@ extern "C" int b200p_session_extend(b200p_session* s, const int* ids, int T, con
     return extend(s, ids, T, want, n_want, logits, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int b200p_session_set_rules(b200p_session* s, const b200p_session_rules* r) {
+extern "C" int b200p_session_set_rules(b200p_session* s, const b200p_session_rules* r) try {
     if (!s) return B200P_E_NULL;
     if (!r) {
         if (s->rules.on) drop_step_graph(s);
@@ -642,7 +643,7 @@ extern "C" int b200p_session_set_rules(b200p_session* s, const b200p_session_rul
     d.bias_n = r->bias_n; d.masked = r->mask != nullptr;
     d.on = true;
     return B200P_OK;
-}
+} catch (const std::bad_alloc&) { return int(cudaErrorMemoryAllocation); }
 
 extern "C" void b200p_session_reset(b200p_session* s) { if (s) s->kv_len = 0; }
 

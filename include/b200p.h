@@ -370,7 +370,7 @@ int b200p_fa_rows_f32(int variant, int bc, const float* Q, const float* K, const
  * host).  With n queries and m keys, causal query i sees the keys j <= m - n + i:
  * the last query sees all, keys beyond the queries are a cache in front of them.
  * A query that sees no key (m < n) gets zeros.  Rows of O outside all sequences
- * are left as they are.  A key that a query does not see does not reach it,
+ * are left as they are; O overlaps no input.  A key that a query does not see does not reach it,
  * whatever it holds (NaN and infinities among it).  Offsets outside the tensors
  * are clamped to them.
  * D 64 or 128, 16-bit I/O, fp32 softmax and accumulation; nQHeads % nKVHeads == 0,
@@ -403,7 +403,7 @@ int b200p_attn_prefill_packed(const void* Q, const void* K, const void* V, const
  * q, o [batch, nQHeads, D]; K_prefix, V_prefix [nKVHeads, prefix_head / D, D];
  * K, V [batch, nKVHeads, own_head / D, D]; lengths: device array of batch ints, each
  * taken into 0 .. max_own, and read on the device, so that a captured launch can be replayed
- * while they grow.  A sequence without any key gets zeros.  Cache rows past a
+ * while they grow; o overlaps no input.  A sequence without any key gets zeros.  Cache rows past a
  * length do not reach the result, whatever they hold. */
 typedef struct b200p_shared_args {
     int D;                     /* head dimension: 64 or 128                               */
@@ -443,7 +443,7 @@ int b200p_attn_decode_shared(const void* q, const void* K_prefix, const void* V_
  * mask_rows[row] says which of them a row takes, a value outside 0 .. n_masks-1 that it
  * takes none; NULL: row i takes mask i.  Every pointer below may be NULL
  * (repetition 1, presence 0, frequency 0, nothing said, no bias, no mask).
- * out may be logits itself (with the same stride). */
+ * out may be logits itself (with the same stride); else the two do not overlap. */
 typedef struct b200p_logits_args {
     int dtype;                 /* B200P_F32, B200P_F16 or B200P_BF16                      */
     int rows;

@@ -215,6 +215,17 @@ def test_offsets_outside_the_tensors_are_clamped(b200p, torch_cuda):
     close(b200p.prefill_packed(Q, K, V, ints(-3, 1000), ints(0, 50), causal=False), want, bound)
 
 
+def test_rows_in_front_of_the_first_sequence(b200p, torch_cuda):
+    torch = torch_cuda
+    Q, K, V, qo, ko = make(torch, [90], [90], 6, 2, 64, torch.bfloat16)
+    out = torch.full_like(Q, 7.0)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    b200p.prefill_packed(Q, K, V, ints(20, 50, 80), ints(10, 40, 70), out=out)
+    want, bound = ref.packed(Q[20:80], K[10:70], V[10:70], [0, 30, 60], [0, 30, 60], True)
+    close(out[20:80], want, bound)
+    assert (out[:20] == 7.0).all() and (out[80:] == 7.0).all()
+
+
 def test_nothing_to_do(b200p, torch_cuda):
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, [0], [0], 4, 2, 64, torch.bfloat16)

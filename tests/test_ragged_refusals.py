@@ -114,12 +114,14 @@ def test_wrappers_check_shapes_first(b200p):
     import torch
     q, K = torch.zeros(4, 8, 64, dtype=torch.bfloat16), torch.zeros(10, 2, 64, dtype=torch.bfloat16)
     n = torch.zeros(3, dtype=torch.int32)
-    for bad in ((q[0], K, K, n, n), (q, K, K[:5], n, n), (q, K[..., :32], K[..., :32], n, n), (q, K, K, n, n[:2]), (q, K, K, n[:0], n[:0]), (q.transpose(1, 2), K, K, n, n), (q.float(), K, K, n, n)):
+    for bad in ((q[0], K, K, n, n), (q, K, K[:5], n, n), (q, K[..., :32], K[..., :32], n, n), (q, K, K, n, n[:2]), (q, K, K, n[:0], n[:0]), (q.transpose(1, 2), K, K, n, n), (q.float(), K, K, n, n),
+                (q[:1].expand(4, 8, 64), K, K, n, n), (q[:1, :1].expand(4, 8, 64), K, K, n, n), (q, K[:1].expand(10, 2, 64), K[:1].expand(10, 2, 64), n, n)):
         with pytest.raises(ValueError):
             b200p._packed_args(*bad, True, 0.0, bad[0])
     Kp, K = torch.zeros(2, 30, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 10, 64, dtype=torch.bfloat16)
     for bad in ((q, Kp, Kp[:, :4], K, K, None), (q, Kp, Kp, K, K, 31), (q, Kp, Kp, K, K, -1), (q, Kp, Kp, K[:3], K[:3], None), (q, Kp[:1], Kp[:1], K, K, None),
-                (q, Kp[:, ::2], Kp[:, ::2], K, K, None), (q, Kp, Kp, K[:, :, ::2], K[:, :, ::2], None), (q[:, ::2], Kp, Kp, K, K, None), (q, Kp, Kp.transpose(0, 1).contiguous().transpose(0, 1), K, K, None)):
+                (q, Kp[:, ::2], Kp[:, ::2], K, K, None), (q, Kp, Kp, K[:, :, ::2], K[:, :, ::2], None), (q[:, ::2], Kp, Kp, K, K, None), (q[:1].expand(4, 8, 64), Kp, Kp, K, K, None), (q, Kp, Kp, K[:1].expand(4, 2, 10, 64), K[:1].expand(4, 2, 10, 64), None),
+                (q, Kp[:1].expand(2, 30, 64), Kp[:1].expand(2, 30, 64), K, K, None), (q, Kp, Kp.transpose(0, 1).contiguous().transpose(0, 1), K, K, None)):
         with pytest.raises(ValueError):
             b200p._shared_args(*bad, 0.0, bad[0])
     b200p._shared_args(q, Kp, Kp, K, K, 7, 0.0, q)
