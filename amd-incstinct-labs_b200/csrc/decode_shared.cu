@@ -10,7 +10,7 @@
 //     (m, l, O) of every split go to the workspace in fp32.  Each tile of the prefix is read once per 256 rows.
 //  2. the sequences' own keys (own_kernel): HBM-bound, every byte of the caches is read once.  A programmatic dependent that
 //     waits for nothing: its CTAs run wherever the first launch leaves room.
-//  3. the merge (merge_kernel).
+//  3. the merge (merge_kernel, packed_launch.cuh).
 // A prefix that is small for its batch is cheaper read per sequence (from L2), by own_kernel, which then is the only launch.
 // ---------------------------------------------------------------------------
 #include "packed_launch.cuh"
@@ -22,8 +22,7 @@ constexpr int kOwnWarps = 4;
 constexpr int kOwnThreads = kOwnWarps * 32;
 constexpr int kKeyBlock = 16;                    // keys of a warp's step
 constexpr int kMostOwnCluster = 8;
-constexpr int kMostSplits = 152;                 // of the prefix: one for each SM, for a single key head
-constexpr int kMostParts = kMostSplits + kMostOwnCluster;
+constexpr int kMostSplits = kMostParts - kMostOwnCluster;        // of the prefix: one for each SM, for a single key head
 
 struct OwnParams {
     const void *q, *Kp, *Vp, *K, *V;
@@ -57,7 +56,6 @@ __device__ __forceinline__ float4 load_cluster_f32x4(uint32_t smem, uint32_t cta
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ float weight_of(float m, float most) { return exp2f(m - (most == -INFINITY ? 0.f : most)); }
 
 // 2^(m_i - m) of this lane's part, m the maximum over the warp, and 1 / sum of 2^(m_i - m) l_i.  A sum of 0 is a part without keys, whose O
 // means nothing.
@@ -304,52 +302,6 @@ own_kernel(const OwnParams p) {
     }
 }
 
-// The parts of a row (the prefix's splits, the CTAs of the sequence's own keys) into its result: a warp per row.
-template <typename T, int D>
-__global__ void __launch_bounds__(kOwnThreads)
-merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int parts, int rows, int nQH, T* __restrict__ o, long long o_batch) {
-    constexpr int E = D / 32;
-    __shared__ float s_f[kOwnWarps][kMostParts];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x * kOwnWarps + warp;
-    griddep_wait();
-    if (row >= rows) return;
-    float2 ml[kMostParts / 32];
-    float most = -INFINITY;
-    #pragma unroll
-    for (int k = 0; k < kMostParts / 32; ++k) {
-        const int s = 32 * k + lane;
-        ml[k] = s < parts ? __ldcg(reinterpret_cast<const float2*>(&part_ml[2 * (size_t(s) * rows + row)])) : make_float2(-INFINITY, 0.f);
-        most = fmaxf(most, ml[k].x);
-    }
-    #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    float sum = 0.f;
-    #pragma unroll
-    for (int k = 0; k < kMostParts / 32; ++k) {
-        const float f = ml[k].y == 0.f ? 0.f : weight_of(ml[k].x, most);
-        sum += f * ml[k].y;
-        if (32 * k + lane < kMostParts) s_f[warp][32 * k + lane] = f;
-    }
-    #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    __syncwarp();
-    float x[E] = {};
-    #pragma unroll 8
-    for (int s = 0; s < parts; ++s) {
-        float v[E];
-        const float* at = part_o + (size_t(s) * rows + row) * D + lane * E;
-        if constexpr (E == 4) { const float4 w = __ldcg(reinterpret_cast<const float4*>(at)); v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w; }
-        else { const float2 w = __ldcg(reinterpret_cast<const float2*>(at)); v[0] = w.x; v[1] = w.y; }
-        const float f = s_f[warp][s];
-        #pragma unroll
-        for (int e = 0; e < E; ++e) if (f != 0.f) x[e] += f * v[e];
-    }
-    const float inv = 1.f / sum;
-    T* y = o + row / nQH * o_batch + (long long)(row % nQH) * D + lane * E;
-    if constexpr (E == 4) *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
-    else *reinterpret_cast<uint32_t*>(y) = pack2<T>(x[0] * inv, x[1] * inv);
-}
-
 // How a call is run.
 struct SharedPlan {
     int splits, span;            // the prefix in a launch of its own: its splits, tiles of an item; 0: none, own_kernel reads the prefix
@@ -411,20 +363,6 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
     return pl;
 }
 
-// A launch that may get ready while the stream's last one runs (it calls griddep_wait for its results).
-template <typename... P, typename... A>
-int launch_after(void (*kern)(P...), dim3 grid, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid; cfg.blockDim = dim3(kOwnThreads); cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-    if (e != cudaSuccess) { cudaGetLastError(); return int(e); }
-    return launched();
-}
-
 template <typename T, int D, int NT>
 int launch_own(const OwnParams& p, int cluster, bool dependent, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
@@ -463,7 +401,7 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
         p.scale_log2 = scale_log2;
         p.q_token = a.q_batch; p.q_head = D; p.k_token = p.v_token = D; p.k_head = p.v_head = a.prefix_head;
         p.part_o = part_o; p.part_ml = part_ml;
-        if (int e = launch_packed<T, D, true>(p, a.dtype, st)) return e;
+        if (int e = launch_packed<T, D, true, false>(p, a.dtype, st)) return e;
     }
     OwnParams w{};
     w.q = q; w.Kp = Kp; w.Vp = Vp; w.K = K; w.V = V; w.o = o; w.lengths = lengths;
@@ -473,9 +411,7 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
     w.scale_log2 = scale_log2; w.apart = apart; w.first_part = pl.splits; w.part_o = part_o; w.part_ml = part_ml;
     if (int e = pl.rows == 8 ? launch_own<T, D, 1>(w, pl.cluster, apart, st) : launch_own<T, D, 2>(w, pl.cluster, apart, st)) return e;
     if (!apart) return B200P_OK;
-    const int rows = a.batch * a.nQHeads;
-    return launch_after(merge_kernel<T, D>, dim3(unsigned((rows + kOwnWarps - 1) / kOwnWarps)), st, static_cast<const float*>(part_o), static_cast<const float*>(part_ml),
-                        pl.splits + pl.cluster, rows, a.nQHeads, static_cast<T*>(o), a.o_batch);
+    return launch_merge<T, D>(part_o, part_ml, pl.splits + pl.cluster, a.batch, a.nQHeads, o, a.o_batch, D, nullptr, nullptr, st);
 }
 
 int checked(const b200p_shared_args* args, b200p_shared_args* out) {

@@ -19,8 +19,10 @@ namespace b200p {
 // The next item is looked for when the K tile of this many steps before the item's end is asked for.  (1, 2, 3, 4: no difference.)
 constexpr int kAskAhead = 2;
 
+constexpr float kNoKey = -1.f;             // in place of a part's sum, whose O is not stored then
+
 struct PackedParams : PrefillParams {      // seqQ, seqK: rows of Q and of K and V; batch: sequences; span, scale_log2, causal, nKVH, group
-    const int *q_offsets, *k_offsets;      // PARTIAL: none, one sequence of all rows
+    const int *q_offsets, *k_offsets;      // without WALK none, one sequence of all rows
     const void *Q, *K, *V;
     void* O;
     long long q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
@@ -28,7 +30,7 @@ struct PackedParams : PrefillParams {      // seqQ, seqK: rows of Q and of K and
     int o_wide;                            // rows of O start on 32 bytes
     int splits;                            // PARTIAL: items that share a block's keys
     float* part_o;                         // PARTIAL: [splits][seqQ][nQH][D]
-    float* part_ml;                        // PARTIAL: [splits][seqQ][nQH][2]: maximum in log2 units, sum; a sum of 0: no key
+    float* part_ml;                        // PARTIAL: [splits][seqQ][nQH][2]: maximum in log2 units, sum; kNoKey for the sum: the row sees no key
 };
 
 // One work item: up to two tiles of one sequence and key head, or a share of their keys.
@@ -55,18 +57,23 @@ __device__ __forceinline__ void packed_tiles_of(const PackedParams& p, int qb, P
     w.nmax = max(w.n[0], w.n[1]);
 }
 
-// PARTIAL: item `id` of the one sequence, a share of a block's keys.
+// PARTIAL: the share of the block's keys that is split w.split.
+__device__ __forceinline__ void packed_share(const PackedParams& p, PackedItem& w) {
+    const int share = (w.nmax + p.splits - 1) / p.splits;
+    w.first = w.split * share;
+    #pragma unroll
+    for (int t = 0; t < 2; ++t) w.n[t] = max(0, min(w.n[t] - w.first, share));
+    w.nmax = max(w.n[0], w.n[1]);
+}
+
+// Without WALK: item `id` of the one sequence.
 __device__ __forceinline__ PackedItem packed_split(const PackedParams& p, int id) {
     PackedItem w{};
     const int rest = id / p.splits, qb = rest / p.nKVH;
     w.split = id - rest * p.splits; w.kvh = rest - qb * p.nKVH;
     w.queries = p.seqQ; w.keys = p.seqK;
     packed_tiles_of(p, qb, w);
-    const int share = (w.nmax + p.splits - 1) / p.splits;
-    w.first = w.split * share;
-    #pragma unroll
-    for (int t = 0; t < 2; ++t) w.n[t] = max(0, min(w.n[t] - w.first, share));
-    w.nmax = max(w.n[0], w.n[1]);
+    packed_share(p, w);
     return w;
 }
 
@@ -76,7 +83,7 @@ template <typename Publish>
 __device__ __forceinline__ bool packed_walk(const PackedParams& p, void* answer, uint64_t* bar, Publish&& publish) {
     constexpr unsigned kAll = 0xffffffffu;
     const int lane = threadIdx.x % 32;
-    const int block = p.span * p.tokens, chunks = (p.batch + 31) / 32;
+    const int block = p.span * p.tokens, chunks = (p.batch + 31) / 32, per = p.nKVH * p.splits;
     int q = 0, k = 0, n = 0, m = 0;                             // this lane's sequence: first rows, lengths
     auto load = [&](int c) {
         const int b = c * 32 + lane;
@@ -125,7 +132,7 @@ __device__ __forceinline__ bool packed_walk(const PackedParams& p, void* answer,
     for (int it = 0;;) {
         PackedItem w{};
         w.kvh = -1;
-        const int entry = id >= 0 ? id / p.nKVH : 0, rest = id - entry * p.nKVH;
+        const int entry = id >= 0 ? id / per : 0, rest = id - entry * per;
         if (id >= 0 && entry >= blocks) {                       // the grid has room for more items than there are
             id = next_id();
             if (id >= 0) continue;
@@ -153,10 +160,11 @@ __device__ __forceinline__ bool packed_walk(const PackedParams& p, void* answer,
             const int within = entry - base;
             const int src = __ffs(__ballot_sync(kAll, upto > within)) - 1;
             const int qb = __shfl_sync(kAll, first + upto - 1 - within, src);       // a sequence's last block of the level first
-            w.kvh = rest;
+            w.kvh = rest / p.splits; w.split = rest - w.kvh * p.splits;
             w.q_row = __shfl_sync(kAll, q, src); w.k_row = __shfl_sync(kAll, k, src);
             w.queries = __shfl_sync(kAll, n, src); w.keys = __shfl_sync(kAll, m, src);
             packed_tiles_of(p, qb, w);
+            if (p.splits > 1) packed_share(p, w);
         }
         const bool go_on = publish(it, w) && w.kvh >= 0;
         ++it;
@@ -189,7 +197,7 @@ template <typename T, typename Sh>
 __device__ __forceinline__ void packed_no_keys(const PackedParams& p, const PackedItem& w, int token, int g) {
     const int head = w.kvh * p.group + g;
     if constexpr (Sh::PARTIAL) {
-        reinterpret_cast<float2*>(p.part_ml)[(size_t(w.split) * p.seqQ + w.q_row + token) * (p.nKVH * p.group) + head] = make_float2(-INFINITY, 0.f);
+        reinterpret_cast<float2*>(p.part_ml)[(size_t(w.split) * p.seqQ + w.q_row + token) * (p.nKVH * p.group) + head] = make_float2(-INFINITY, kNoKey);
     } else {
         uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(p.O) + (w.q_row + token) * p.o_token + head * p.o_head);
         for (int i = 0; i < Sh::DV / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
@@ -214,7 +222,7 @@ __device__ __forceinline__ void packed_epilogue(const PackedParams& p, const Pac
     unsigned char* mine = nullptr;
     if constexpr (PARTIAL) {
         const size_t row = (size_t(w.split) * p.seqQ + w.q_row + token) * (p.nKVH * p.group) + w.kvh * p.group + g;
-        if (live) reinterpret_cast<float2*>(p.part_ml)[row] = sees ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        if (live) reinterpret_cast<float2*>(p.part_ml)[row] = sees ? make_float2(m, l) : make_float2(-INFINITY, kNoKey);
         if (sees) mine = reinterpret_cast<unsigned char*>(p.part_o + row * D);
     } else if (live) mine = reinterpret_cast<unsigned char*>(static_cast<T*>(p.O) + (w.q_row + token) * p.o_token + (w.kvh * p.group + g) * p.o_head);
     if (mine) {

@@ -9,16 +9,16 @@ namespace b200p {
 inline long long packed_tiles(long long rows, int batch, int tokens, int kv_heads) { return (rows / tokens + batch) * kv_heads; }
 
 // Everything of p but the launch's own fields (tokens, sticky; span where it is 0) is set.
-template <typename T, int D, bool PARTIAL>
+template <typename T, int D, bool PARTIAL, bool WALK>
 int launch_packed(PackedParams p, int dtype, cudaStream_t st) {
-    using Sh = PackedShape<D, PARTIAL>;
+    using Sh = PackedShape<D, PARTIAL, WALK>;
     const CUtensorMapDataType dt = dtype == B200P_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     p.tokens = kBM / p.group;
     const int sms = sm_count();
     const long long tiles = packed_tiles(p.seqQ, p.batch, p.tokens, p.nKVH) * p.splits;
     if (p.span == 0) p.span = tiles <= sms ? 1 : 2;            // a tile alone takes 0.6 of a pair's time (prefill.cu)
     const int block = p.span * p.tokens;
-    const long long items = PARTIAL ? (long long)((p.seqQ + block - 1) / block) * p.nKVH * p.splits : packed_tiles(p.seqQ, p.batch, block, p.nKVH);
+    const long long items = (WALK ? packed_tiles(p.seqQ, p.batch, block, p.nKVH) : (long long)((p.seqQ + block - 1) / block) * p.nKVH) * p.splits;
     if (items > (1 << 29)) return B200P_E_RANGE;
     CUtensorMap mq, mk, mv;
     auto rows_map = [&](CUtensorMap* m, const void* base, long long token, long long head) {      // [head of a group][token][group]
@@ -43,10 +43,89 @@ int launch_packed(PackedParams p, int dtype, cudaStream_t st) {
     p.sticky = device_status_ptr();
     if (!p.sticky) return B200P_E_NO_DEVICE;
     p.items = int(items);
-    // PARTIAL items are alike, and a launch that waits for this one comes behind them: a CTA per SM with a fixed share
-    const long long ctas = PARTIAL && items > sms ? sms : items;
+    // the items of one sequence are alike: a CTA per SM with a fixed share
+    const long long ctas = !WALK && items > sms ? sms : items;
     kern<<<unsigned(ctas), prefill_threads(1), Sh::SMEM_BYTES, st>>>(p, mq, mk, mv, mq, mq, mk);
     return launched();
+}
+
+// ---- parts of rows (the splits' results) into the rows' results ------------------------------------------
+constexpr int kMostParts = 160;
+constexpr int kMergeWarps = 4;
+
+__device__ __forceinline__ float weight_of(float m, float most) { return exp2f(m - (most == -INFINITY ? 0.f : most)); }
+
+// Row r = token * nQH + head from part_o[s][r][D] and part_ml[s][r]: a warp per row.  m = max m_s, O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s;
+// parts without a key do not count, a row without any gives zeros.  first, last: device words with the first row to be written and the one
+// behind the last, in tokens, or null.
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32)
+merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int parts, int tokens, int nQH, T* __restrict__ o, long long o_token, long long o_head,
+             const int* first, const int* last) {
+    constexpr int E = D / 32;
+    __shared__ float s_f[kMergeWarps][kMostParts];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x * kMergeWarps + warp, rows = tokens * nQH, token = row / nQH;
+    griddep_wait();
+    if (row >= rows || (first && (token < *first || token >= *last))) return;
+    float2 ml[kMostParts / 32];
+    float most = -INFINITY;
+    bool some = false;
+    #pragma unroll
+    for (int k = 0; k < kMostParts / 32; ++k) {
+        const int s = 32 * k + lane;
+        ml[k] = s < parts ? __ldcg(reinterpret_cast<const float2*>(&part_ml[2 * (size_t(s) * rows + row)])) : make_float2(-INFINITY, kNoKey);
+        most = fmaxf(most, ml[k].x);
+        some |= ml[k].y != kNoKey;
+    }
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    some = __any_sync(0xffffffffu, some);
+    float sum = 0.f;
+    #pragma unroll
+    for (int k = 0; k < kMostParts / 32; ++k) {
+        const float f = ml[k].y <= 0.f ? 0.f : weight_of(ml[k].x, most);        // no key, or nothing but scores of -inf
+        sum += f == 0.f ? 0.f : f * ml[k].y;
+        s_f[warp][32 * k + lane] = f;
+    }
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    __syncwarp();
+    float x[E] = {};
+    #pragma unroll 8
+    for (int s = 0; s < parts; ++s) {
+        float v[E];
+        const float* at = part_o + (size_t(s) * rows + row) * D + lane * E;
+        if constexpr (E == 4) { const float4 w = __ldcg(reinterpret_cast<const float4*>(at)); v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w; }
+        else { const float2 w = __ldcg(reinterpret_cast<const float2*>(at)); v[0] = w.x; v[1] = w.y; }
+        const float f = s_f[warp][s];
+        #pragma unroll
+        for (int e = 0; e < E; ++e) if (f != 0.f) x[e] += f * v[e];
+    }
+    const float inv = some ? 1.f / sum : 0.f;               // nothing but scores of -inf: 0 / 0
+    T* y = o + token * o_token + (row - token * nQH) * o_head + lane * E;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
+    else *reinterpret_cast<uint32_t*>(y) = pack2<T>(x[0] * inv, x[1] * inv);
+}
+
+// A launch that may get ready while the stream's last one runs (it calls griddep_wait for its results).
+template <typename... P, typename... A>
+int launch_after(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(unsigned(threads)); cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) { cudaGetLastError(); return int(e); }
+    return launched();
+}
+
+template <typename T, int D>
+int launch_merge(const float* part_o, const float* part_ml, int parts, int tokens, int nQH, void* o, long long o_token, long long o_head, const int* first, const int* last,
+                 cudaStream_t st) {
+    const long long ctas = ((long long)tokens * nQH + kMergeWarps - 1) / kMergeWarps;
+    return launch_after(merge_kernel<T, D>, dim3(unsigned(ctas)), kMergeWarps * 32, st, part_o, part_ml, parts, tokens, nQH, static_cast<T*>(o), o_token, o_head, first, last);
 }
 
 } // namespace b200p

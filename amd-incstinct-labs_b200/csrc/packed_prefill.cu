@@ -6,16 +6,48 @@
 namespace b200p {
 namespace {
 
+// In how many splits the keys are taken, for few query tiles with many keys (a few new tokens on a long cache): a tile takes 1.35 us per
+// 128 keys, one after the other; the parts' way through the workspace and the merge take 4 us.  A split has two key tiles at least, going by
+// the mean, and there are no more than SMs: a second round of items costs what it was to save.  (Without and with, heads of 128: 16 tokens on 8000 keys, 32 / 8 heads, 101 and 17.5 us;
+// 8 single tokens on 8000 keys 101 and 60; 64 tokens, 1024 keys, 19.1 and 13.6; 300 tokens, 300 keys, 10.3 and, with 2 splits, 11.4: under 1024
+// keys none.)
+struct PackedPlan { int splits; size_t off_ml, ws_bytes; };
+PackedPlan plan_packed(const b200p_packed_args& a) {
+    PackedPlan pl{1, 0, 0};
+    if (a.batch == 0 || a.total_q == 0) return pl;
+    const int sms = sm_count() > 0 ? sm_count() : 148, group = a.nQHeads / a.nKVHeads;
+    const int tokens = kBM / group;
+    const long long about = a.total_q / tokens + (a.batch + 1) / 2;            // of a key head: every second sequence fills a tile more than its share
+    const long long tiles = (about > a.batch ? about : a.batch) * a.nKVHeads, keys = a.total_k / a.batch;
+    const int fixed = tuning(KNOB_PACKED_SPLITS, 0);
+    if (fixed > 0) pl.splits = fixed < kMostParts ? fixed : kMostParts;
+    else if (keys >= 8 * kBN && 2 * tiles <= sms) {
+        const long long s = sms / tiles, most = (keys + 2 * kBN - 1) / (2 * kBN);
+        pl.splits = int(s < most ? s : most);
+        if (pl.splits > kMostParts) pl.splits = kMostParts;
+    }
+    if (pl.splits > 1) {
+        const size_t all = size_t(pl.splits) * a.total_q * a.nQHeads;
+        pl.off_ml = (all * a.D * 4 + 255) / 256 * 256;
+        pl.ws_bytes = pl.off_ml + (all * 8 + 255) / 256 * 256;
+    }
+    return pl;
+}
+
 template <typename T, int D>
-int launch(const void* Q, const void* K, const void* V, const int* qo, const int* ko, void* O, const b200p_packed_args& a, cudaStream_t st) {
+int launch(const void* Q, const void* K, const void* V, const int* qo, const int* ko, void* O, const b200p_packed_args& a, const PackedPlan& pl, void* workspace, cudaStream_t st) {
     PackedParams p{};
     p.Q = Q; p.K = K; p.V = V; p.O = O; p.q_offsets = qo; p.k_offsets = ko;
     p.seqQ = a.total_q; p.seqK = a.total_k; p.batch = a.batch; p.causal = a.causal != 0;
-    p.nQH = a.nQHeads; p.nKVH = a.nKVHeads; p.group = a.nQHeads / a.nKVHeads; p.splits = 1;
+    p.nQH = a.nQHeads; p.nKVH = a.nKVHeads; p.group = a.nQHeads / a.nKVHeads; p.splits = pl.splits;
     p.scale_log2 = 1.4426950408889634f * (a.scale > 0.f ? a.scale : 1.f / sqrtf(float(D)));
     p.q_token = a.q_token; p.q_head = a.q_head; p.k_token = a.k_token; p.k_head = a.k_head;
     p.v_token = a.v_token; p.v_head = a.v_head; p.o_token = a.o_token; p.o_head = a.o_head;
-    return launch_packed<T, D, false>(p, a.dtype, st);
+    if (pl.splits == 1) return launch_packed<T, D, false, true>(p, a.dtype, st);
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pl.off_ml);
+    if (int e = launch_packed<T, D, true, true>(p, a.dtype, st)) return e;
+    return launch_merge<T, D>(p.part_o, p.part_ml, pl.splits, a.total_q, a.nQHeads, O, a.o_token, a.o_head, qo, qo + a.batch, st);
 }
 
 // Checks what the entry points share and fills in the dense strides.
@@ -26,7 +58,7 @@ int checked(const b200p_packed_args* args, b200p_packed_args* out) {
     if (a.D != 64 && a.D != 128) return B200P_E_DIM;
     if (a.nQHeads <= 0 || a.nKVHeads <= 0 || a.nQHeads % a.nKVHeads != 0) return B200P_E_DIM;
     if (a.batch < 0 || a.total_q < 0 || a.total_k < 0 || !(a.scale >= 0.f) || std::isinf(a.scale)) return B200P_E_LENGTH;
-    if (a.nQHeads / a.nKVHeads > 128 || a.nQHeads > 65535 || a.batch > (1 << 24)) return B200P_E_RANGE;
+    if (a.nQHeads / a.nKVHeads > 128 || a.nQHeads > 65535 || a.batch > (1 << 24) || (long long)a.total_q * a.nQHeads > 0x7fffffffLL) return B200P_E_RANGE;
     const long long D = a.D;
     auto fill = [&](long long& token, long long& head, long long heads) { if (token == 0 && head == 0) { token = heads * D; head = D; } };
     fill(a.q_token, a.q_head, a.nQHeads); fill(a.k_token, a.k_head, a.nKVHeads); fill(a.v_token, a.v_head, a.nKVHeads); fill(a.o_token, a.o_head, a.nQHeads);
@@ -46,8 +78,8 @@ int checked(const b200p_packed_args* args, b200p_packed_args* out) {
 using namespace b200p;
 
 extern "C" size_t b200p_attn_prefill_packed_workspace_bytes(const b200p_packed_args* args) {
-    (void)args;
-    return 0;
+    b200p_packed_args a;
+    return checked(args, &a) == B200P_OK ? plan_packed(a).ws_bytes : 0;
 }
 
 extern "C" int b200p_attn_prefill_packed(const void* Q, const void* K, const void* V, const int* q_offsets, const int* k_offsets, void* O,
@@ -58,7 +90,13 @@ extern "C" int b200p_attn_prefill_packed(const void* Q, const void* K, const voi
     if (!Q || !O || !q_offsets || !k_offsets || (a.total_k > 0 && (!K || !V))) return B200P_E_NULL;
     if (!aligned(Q, 16) || !aligned(K, 16) || !aligned(V, 16) || !aligned(O, 16) || !aligned(q_offsets, 4) || !aligned(k_offsets, 4)) return B200P_E_ALIGN;
     if (sm_count() <= 0) return B200P_E_NO_DEVICE;
+    const PackedPlan pl = plan_packed(a);
+    if (pl.ws_bytes > 0 && (!workspace || workspace_bytes < pl.ws_bytes)) return B200P_E_WORKSPACE;
+    if (!aligned(workspace, 256)) return B200P_E_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.dtype == B200P_F16) return a.D == 128 ? launch<__half, 128>(Q, K, V, q_offsets, k_offsets, O, a, st) : launch<__half, 64>(Q, K, V, q_offsets, k_offsets, O, a, st);
-    return a.D == 128 ? launch<__nv_bfloat16, 128>(Q, K, V, q_offsets, k_offsets, O, a, st) : launch<__nv_bfloat16, 64>(Q, K, V, q_offsets, k_offsets, O, a, st);
+    auto run = [&](auto tag) -> int {
+        using T = decltype(tag);
+        return a.D == 128 ? launch<T, 128>(Q, K, V, q_offsets, k_offsets, O, a, pl, workspace, st) : launch<T, 64>(Q, K, V, q_offsets, k_offsets, O, a, pl, workspace, st);
+    };
+    return a.dtype == B200P_F16 ? run(__half{}) : run(__nv_bfloat16{});
 }

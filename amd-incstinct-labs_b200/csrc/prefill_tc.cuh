@@ -82,27 +82,28 @@ template <int QKS, int VS, int KST, int VST, int OCOLS> struct PrefillTiles {
 struct PrefillParams;
 struct PackedParams;
 template <int D> struct PrefillShape : PrefillTiles<D / 64, D / 64, (D == 128) ? 2 : 4, (D == 128) ? 2 : 4, 64> {
-    static constexpr bool LATENT = false, PORTION = false, MASKED = false, PACKED = false, PARTIAL = false;
+    static constexpr bool LATENT = false, PORTION = false, MASKED = false, PACKED = false, PARTIAL = false, WALK = false;
     using Params = PrefillParams;
 };
 // PACKED: sequences of different lengths, one after the other in token-major tensors (packed.cuh).  A tile's rows are the heads
 // of a group of `tokens` tokens, so that the keys of a group are read once for all its heads and short sequences fill a tile.
 // PARTIAL: a tile's keys may be split between items; O, not yet divided, and the row's maximum and sum go to a workspace in fp32.
-template <int D, bool PART> struct PackedShape : PrefillTiles<D / 64, D / 64, (D == 128) ? 2 : 4, (D == 128) ? 2 : 4, 64> {
-    static constexpr bool LATENT = false, PORTION = false, MASKED = false, PACKED = true, PARTIAL = PART;
+// WALK: the sequences' offsets are looked at; without it, one sequence of all rows.
+template <int D, bool PART, bool OFFSETS> struct PackedShape : PrefillTiles<D / 64, D / 64, (D == 128) ? 2 : 4, (D == 128) ? 2 : 4, 64> {
+    static constexpr bool LATENT = false, PORTION = false, MASKED = false, PACKED = true, PARTIAL = PART, WALK = OFFSETS;
     using Params = PackedParams;
 };
 // PORTION: causal with an offset (a portion of a prompt starts behind the cached tokens), value columns that need not fill
 // their boxes, an optional sink in the softmax.  MASKED: a row also has a first key (AttnMask), key tiles before the first
 // row's are skipped.  Grouped heads, keys and values of different widths (grouped_attn.cuh).
 template <int QKS, int VS> struct MaskedPrefillShape : PrefillTiles<QKS, VS, (QKS + VS > 2) ? 2 : 4, (QKS + VS > 2) ? 2 : 4, 64> {
-    static constexpr bool LATENT = false, PORTION = true, MASKED = true, PACKED = false, PARTIAL = false;
+    static constexpr bool LATENT = false, PORTION = true, MASKED = true, PACKED = false, PARTIAL = false, WALK = false;
     using Params = PrefillParams;
 };
 // Latent attention on expanded keys and values (latent.cuh): PLAIN boxes of a query / key row without positions, then
 // one box of the rotated part, which has its own tensor maps (the key's is the same for all heads).
 template <int PLAIN, int VS> struct LatentPrefillShape : PrefillTiles<PLAIN + 1, VS, (PLAIN + VS > 2) ? 1 : 2, 2, 32> {
-    static constexpr bool LATENT = true, PORTION = true, MASKED = false, PACKED = false, PARTIAL = false;
+    static constexpr bool LATENT = true, PORTION = true, MASKED = false, PACKED = false, PARTIAL = false, WALK = false;
     using Params = PrefillParams;
 };
 
@@ -168,7 +169,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                   const __grid_constant__ CUtensorMap mapO, const __grid_constant__ CUtensorMap mapQr,
                   const __grid_constant__ CUtensorMap mapKr) {
     constexpr int DV = Sh::DV;
-    constexpr bool LATENT = Sh::LATENT, PORTION = Sh::PORTION, MASKED = Sh::MASKED, PACKED = Sh::PACKED, PARTIAL = Sh::PARTIAL;
+    constexpr bool LATENT = Sh::LATENT, PORTION = Sh::PORTION, MASKED = Sh::MASKED, PACKED = Sh::PACKED, WALK = Sh::WALK;
     constexpr int KST = Sh::KSTAGES, VST = Sh::VSTAGES;
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::OFF_BAR);
@@ -195,7 +196,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
 
     constexpr int kMmaWarp = 8 * RS, kTmaWarp = 8 * RS + 1, kWalkWarp = 8 * RS + 2;
     constexpr int kItemReaders = 2 * kBM + 1 + PACKED;         // every softmax thread + the MMA thread; PACKED: + the TMA thread
-    if constexpr (PARTIAL) griddep_launch_dependents();        // the merge that follows may get ready
+    if constexpr (PACKED && !WALK) griddep_launch_dependents();       // what follows may get ready, or begin beside
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
@@ -227,7 +228,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
     // publishes them whole.
     int* const abort_word = [&] { if constexpr (PACKED) return &s_failed; else return p.status; }();     // PACKED: no CTA waits for another
     auto read_item = [&](int it, Item& w) -> int {             // behind item_full: the CTA's it-th item; its id, or negative: there are no more
-        if constexpr (PARTIAL) {                               // known without looking: every role finds them itself
+        if constexpr (PACKED && !WALK) {                       // known without looking: every role finds them itself
             const int id = int(blockIdx.x) + it * int(gridDim.x);
             if (id >= p.items) return -1;
             w = packed_split(p, id);
@@ -239,9 +240,9 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         }
     };
     auto next_item = [&](int it, Item& w) -> int {             // consumer side
-        if (!PARTIAL && !dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word)) return -2;
+        if (!(PACKED && !WALK) && !dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word)) return -2;
         const int id = read_item(it, w);
-        if (!PARTIAL) dme::mbar_arrive(&item_empty[it & 1]);
+        if (!(PACKED && !WALK)) dme::mbar_arrive(&item_empty[it & 1]);
         return id;
     };
 
@@ -348,11 +349,11 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         int worked = 0;                // PACKED: earlier items with keys: phase of q_full
         bool ok = true;
         for (int it = 0; ok; ++it) {
-            if (!PARTIAL && !wait(&item_full[it & 1], uint32_t((it >> 1) & 1))) { ok = false; break; }
+            if (!(PACKED && !WALK) && !wait(&item_full[it & 1], uint32_t((it >> 1) & 1))) { ok = false; break; }
             Item w;
             const int id = __shfl_sync(0xffffffffu, read_item(it, w), 0);
             if constexpr (PACKED) __syncwarp();                  // all lanes have read the item
-            if (!PARTIAL) { if (tc::elect_one()) dme::mbar_arrive(&item_empty[it & 1]); }
+            if (!(PACKED && !WALK)) { if (tc::elect_one()) dme::mbar_arrive(&item_empty[it & 1]); }
             __syncwarp();
             if (id < 0) break;
             if constexpr (PACKED) {
@@ -437,8 +438,8 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
             cs0 += n0; cs1 += n1; co0 += n0 > 0; co1 += n1 > 0;
         }
         if (!ok && lane == 0) atomicExch(&s_failed, 1);
-      } else if (PACKED && !PARTIAL && warp == kWalkWarp) {
-        if constexpr (PACKED && !PARTIAL) {
+      } else if (WALK && warp == kWalkWarp) {
+        if constexpr (WALK) {
             bool ok = true;
             const bool fine = packed_walk(p, s_answer, answer_bar, [&](int it, const PackedItem& w) -> bool {
                 if (it >= 2) ok = dme::wait(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1), abort_word);

@@ -26,6 +26,14 @@ def close(got, want, bound):
     assert (off <= bound).all(), worst
 
 
+@pytest.fixture(params=[-1, 2, 7], ids=["chosen", "2 splits", "7 splits"])
+def splits(b200p, request):
+    """The keys as the sizes choose, and split."""
+    b200p.set_tuning("packed_splits", request.param)
+    yield request.param
+    b200p.set_tuning("packed_splits", -1)
+
+
 KINDS = {"bf16": "bfloat16", "f16": "float16"}
 HEADS = [(8, 2), (4, 4), (6, 2), (5, 1), (16, 1), (7, 7)]
 LENGTHS = [[1], [128], [129], [64, 1, 65], [20, 0, 300, 1], [0, 17, 0, 0], [257, 128, 127], [1] * 40, [513]]
@@ -49,7 +57,7 @@ def test_prompts(b200p, torch_cuda, i, D, causal, kind):
 @pytest.mark.parametrize("heads,kv,D", [(8, 2, 128), (8, 1, 64), (3, 1, 128), (4, 4, 64), (12, 1, 128)])
 @pytest.mark.parametrize("new,keys", [([5, 1, 40], [133, 700, 40]), ([1, 1, 1], [1, 128, 1000]), ([30, 200], [7, 129]), ([9, 3, 150], [0, 3, 0]), ([0, 2, 0], [50, 2, 300]),
                                       ([300], [1400]), ([64] * 9, [128 * i for i in range(9)])])
-def test_keys_in_front_of_the_queries(b200p, torch_cuda, new, keys, heads, kv, D, causal):
+def test_keys_in_front_of_the_queries(b200p, torch_cuda, splits, new, keys, heads, kv, D, causal):
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, new, keys, heads, kv, D, torch.bfloat16, seed=len(new))
     got = b200p.prefill_packed(Q, K, V, qo, ko, causal=causal)
@@ -60,11 +68,24 @@ def test_keys_in_front_of_the_queries(b200p, torch_cuda, new, keys, heads, kv, D
 
 
 @pytest.mark.parametrize("batch", [33, 1100])
-def test_many_sequences(b200p, torch_cuda, batch):
+def test_many_sequences(b200p, torch_cuda, splits, batch):
     torch = torch_cuda
     new = [(i * 37) % 90 for i in range(batch)]
     Q, K, V, qo, ko = make(torch, new, new, 4, 2, 64, torch.bfloat16)
     close(b200p.prefill_packed(Q, K, V, qo), *ref.packed(Q, K, V, at(new), at(new), True))
+
+
+# few queries on long caches: split without being told
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("new,keys,heads,kv,D", [([16], [8000], 32, 8, 128), ([1] * 8, [5000 + 300 * i for i in range(8)], 8, 2, 64), ([64, 3], [1024, 3000], 6, 1, 128), ([130], [9000], 4, 4, 64),
+                                                 ([5, 0, 7], [4000, 200, 0], 8, 8, 128), ([2000], [2000], 1, 1, 64)])
+def test_few_queries_on_long_caches(b200p, torch_cuda, new, keys, heads, kv, D, kind):
+    torch = torch_cuda
+    Q, K, V, qo, ko = make(torch, new, keys, heads, kv, D, getattr(torch, KINDS[kind]))
+    assert b200p.prefill_packed_workspace(Q, K, V, qo, ko).numel() > 0
+    got = b200p.prefill_packed(Q, K, V, qo, ko)
+    assert b200p.device_status() == 0
+    close(got, *ref.packed(Q, K, V, at(new), at(keys), True))
 
 
 def test_more_work_than_one_round_of_the_device(b200p, torch_cuda):
@@ -75,7 +96,7 @@ def test_more_work_than_one_round_of_the_device(b200p, torch_cuda):
 
 
 @pytest.mark.parametrize("scale", [0.01, 1.0])
-def test_scale_and_large_scores(b200p, torch_cuda, scale):
+def test_scale_and_large_scores(b200p, torch_cuda, splits, scale):
     torch = torch_cuda
     new = [200, 31]
     Q, K, V, qo, ko = make(torch, new, new, 4, 2, 64, torch.bfloat16, size=4.0)
@@ -85,7 +106,7 @@ def test_scale_and_large_scores(b200p, torch_cuda, scale):
 # one projection's rows hold Q, K and V of all heads; head-major tensors; O in a wider buffer
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("layout", ["fused", "head_major"])
-def test_strided_views(b200p, torch_cuda, layout, D):
+def test_strided_views(b200p, torch_cuda, splits, layout, D):
     torch = torch_cuda
     g = torch.Generator(device="cuda").manual_seed(3)
     new, heads, kv = [70, 3, 200], 6, 2
@@ -110,7 +131,7 @@ def test_strided_views(b200p, torch_cuda, layout, D):
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("D", [64, 128])
-def test_what_is_not_seen_does_not_reach_a_query(b200p, torch_cuda, D, causal, bad):
+def test_what_is_not_seen_does_not_reach_a_query(b200p, torch_cuda, splits, D, causal, bad):
     torch = torch_cuda
     new, heads, kv = [100, 130, 40], 4, 2
     Q, K, V, qo, ko = make(torch, new + [50], new + [50], heads, kv, D, torch.bfloat16)
@@ -129,7 +150,7 @@ def test_what_is_not_seen_does_not_reach_a_query(b200p, torch_cuda, D, causal, b
     assert not got[265:270].isfinite().any()
 
 
-def test_values_that_are_infinite_where_they_are_seen(b200p, torch_cuda):
+def test_values_that_are_infinite_where_they_are_seen(b200p, torch_cuda, splits):
     """An infinite value is the answer of every query that sees it, in its column alone."""
     torch = torch_cuda
     new = [150]
@@ -143,7 +164,7 @@ def test_values_that_are_infinite_where_they_are_seen(b200p, torch_cuda):
     close(got[:, :, keep], want[:, :, keep], bound[:, :, keep])
 
 
-def test_scores_that_overflow(b200p, torch_cuda):
+def test_scores_that_overflow(b200p, torch_cuda, splits):
     """Visible scores of -inf weigh nothing; a row of nothing but -inf has no answer."""
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, [140], [140], 2, 2, 64, torch.bfloat16)
@@ -155,7 +176,7 @@ def test_scores_that_overflow(b200p, torch_cuda):
     assert got[:135].isnan().all()
 
 
-def test_same_bits_again_and_on_another_stream(b200p, torch_cuda):
+def test_same_bits_again_and_on_another_stream(b200p, torch_cuda, splits):
     torch = torch_cuda
     new = [300, 77, 1000, 5]
     Q, K, V, qo, ko = make(torch, new, new, 8, 2, 128, torch.bfloat16)
@@ -174,7 +195,7 @@ def test_same_bits_again_and_on_another_stream(b200p, torch_cuda):
     close(alone, want[377:1377], bound[377:1377])
 
 
-def test_captured_and_replayed_with_other_lengths(b200p, torch_cuda):
+def test_captured_and_replayed_with_other_lengths(b200p, torch_cuda, splits):
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, [400], [400], 4, 2, 64, torch.bfloat16)
     qo = torch.tensor([0, 100, 400], dtype=torch.int32, device="cuda")
@@ -206,7 +227,7 @@ def test_offsets_past_32_bits(b200p, torch_cuda):
     close(got, want, bound)
 
 
-def test_offsets_outside_the_tensors_are_clamped(b200p, torch_cuda):
+def test_offsets_outside_the_tensors_are_clamped(b200p, torch_cuda, splits):
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, [50], [50], 2, 1, 64, torch.bfloat16)
     want, bound = ref.packed(Q, K, V, [0, 50], [0, 50], False)
@@ -215,7 +236,7 @@ def test_offsets_outside_the_tensors_are_clamped(b200p, torch_cuda):
     close(b200p.prefill_packed(Q, K, V, ints(-3, 1000), ints(0, 50), causal=False), want, bound)
 
 
-def test_rows_in_front_of_the_first_sequence(b200p, torch_cuda):
+def test_rows_in_front_of_the_first_sequence(b200p, torch_cuda, splits):
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, [90], [90], 6, 2, 64, torch.bfloat16)
     out = torch.full_like(Q, 7.0)
@@ -226,7 +247,7 @@ def test_rows_in_front_of_the_first_sequence(b200p, torch_cuda):
     assert (out[:20] == 7.0).all() and (out[80:] == 7.0).all()
 
 
-def test_nothing_to_do(b200p, torch_cuda):
+def test_nothing_to_do(b200p, torch_cuda, splits):
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, [0], [0], 4, 2, 64, torch.bfloat16)
     assert b200p.prefill_packed(Q, K, V, qo).shape == (0, 4, 64)

@@ -38,6 +38,8 @@ def test_packed_pointers(b200p):
     assert call_packed(b200p, packed(b200p, batch=0), Q=None, O=None) == 0
     assert call_packed(b200p, packed(b200p, total_q=0), Q=None, O=None) == 0
     assert b200p.lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(packed(b200p, D=96))) == 0
+    assert b200p.lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(packed(b200p, total_q=5000))) == 0
+    assert b200p.lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(packed(b200p, total_q=3, total_k=30000))) > 0
 
 
 def shared(b200p, **more):
