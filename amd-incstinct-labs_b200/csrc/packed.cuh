@@ -5,7 +5,8 @@
 //    32 sequences at a time, and finds the CTA's items by number.  Items are numbered by falling number of key tiles; the grid has
 //    a CTA for each of them, and a CTA that is done takes over the next one's number from the hardware (launch_control.cuh): the
 //    heaviest items first, no SM idle while there are others, no counter in memory to clear ahead of a launch or to share.
-//  * its rows.  A tile holds the heads of a group for 128 / group tokens, token by token.
+//  * its rows.  A tile holds the heads of a group for 128 / group tokens, token by token: keys are read once for a group, a
+//    prompt of 20 tokens fills 80 rows of a tile with 4 heads to a group, and the causal mask costs no more tiles than it would by head.
 //  * what happens to rows that are no numbers.  A weight of zero times a value that is none (behind a causal row's position in
 //    its key tile) gives none, and so does a tile of nothing but -inf scores ahead of finite ones.  Rows with such a result are done
 //    again key by key (attn_rows.cuh), from those keys alone that the row sees.

@@ -1,5 +1,13 @@
 // ---------------------------------------------------------------------------
-// packed_prefill.cu -- attention of prompts of different lengths that lie one after the other in one tensor.
+// packed_prefill.cu -- attention of prompts of different lengths that lie one after the other in one tensor: row i of a
+// sequence with n queries and m keys is softmax(scale q_i K^T) V over the keys j <= m - n + i (causal) or all m.
+//
+// The tcgen05 prefill kernel (prefill_tc.cuh) in its packed form (packed.cuh): one pass over the keys with the running maximum
+// and sum, S and O in tensor memory.  Bound by the softmax warps' own instruction stream, as the dense form is: a step of 128 keys
+// takes two query tiles 1.7 us whether heads are 64 or 128 wide, and an item 3 us more for its first S and its way out.  Measured, calls replayed
+// from a graph: 8 documents of 2000 to 8192 tokens, 32 / 8 heads of 128, bf16, causal, 2.35 ms = 1073 TFLOP/s (0.65 of the GEMM's burst);
+// 16 prompts of 100 to 1500 tokens 100 us = 748; 27 texts of 0 to 900, 32 / 4 heads of 64, fp16, not causal, 42 to 46 us = 370; 6 portions of
+// 120 to 512 tokens on up to 6500 cached keys 127 us = 904; two questions of 19 and 40 tokens 7.2 us.
 // ---------------------------------------------------------------------------
 #include "packed_launch.cuh"
 
@@ -8,8 +16,8 @@ namespace {
 
 // In how many splits the keys are taken, for few query tiles with many keys (a few new tokens on a long cache): a tile takes 1.35 us per
 // 128 keys, one after the other; the parts' way through the workspace and the merge take 4 us.  A split has two key tiles at least, going by
-// the mean, and there are no more than SMs: a second round of items costs what it was to save.  (Without and with, heads of 128: 16 tokens on 8000 keys, 32 / 8 heads, 101 and 17.5 us;
-// 8 single tokens on 8000 keys 101 and 60; 64 tokens, 1024 keys, 19.1 and 13.6; 300 tokens, 300 keys, 10.3 and, with 2 splits, 11.4: under 1024
+// the mean, and there are no more than SMs: a second round of items costs what it was to save.  (Without and with, 32 / 8 heads of 128:
+// 16 tokens on 8000 keys 101 and 17.5 us; 8 single tokens on 8000 keys 101 and 60; 64 tokens, 1024 keys, 19.1 and 13.6; 300 tokens, 300 keys, 10.3 and, with 2 splits, 11.4: under 1024
 // keys none.)
 struct PackedPlan { int splits; size_t off_ml, ws_bytes; };
 PackedPlan plan_packed(const b200p_packed_args& a) {

@@ -379,7 +379,8 @@ typedef struct b200p_packed_args {
     int D;
     int nQHeads;
     int nKVHeads;
-    int batch;                 /* sequences; empty ones (no queries, no keys) are fine    */
+    int batch;                 /* sequences, at most 2^24; empty ones (no queries, no keys)
+                                  are fine                                                */
     int total_q, total_k;      /* rows of Q and O, rows of K and V                        */
     int causal;
     int dtype;                 /* B200P_F16 or B200P_BF16                                 */
@@ -409,7 +410,7 @@ typedef struct b200p_shared_args {
     int D;                     /* head dimension: 64 or 128                               */
     int nQHeads;
     int nKVHeads;              /* nQHeads % nKVHeads == 0, at most 128 per key head       */
-    int batch;
+    int batch;                 /* sequences, at most 65535                                */
     int prefix_len;            /* keys of the prefix, may be 0                            */
     int max_own;               /* bound of lengths[], may be 0                            */
     int dtype;                 /* B200P_F16 or B200P_BF16                                 */
@@ -446,8 +447,8 @@ int b200p_attn_decode_shared(const void* q, const void* K_prefix, const void* V_
  * out may be logits itself (with the same stride); else the two do not overlap. */
 typedef struct b200p_logits_args {
     int dtype;                 /* B200P_F32, B200P_F16 or B200P_BF16                      */
-    int rows;
-    int vocab;
+    int rows;                  /* at most 65535                                           */
+    int vocab;                 /* at most 2^30                                            */
     int prompt_max, tokens_max;
     int bias_n;                /* entries of a row's bias list, at most 1024              */
     int n_masks;
