@@ -587,6 +587,10 @@ def _on(device, call, *args):
         return call(*args)
 
 
+def _expanded(*shapes_and_strides):
+    return any(stride == 0 and n > 1 for shape, strides in shapes_and_strides for n, stride in zip(shape, strides))
+
+
 def _scratch(workspace, size, a, like, device):
     """The caller's workspace, or one made for this call, of the size that the library asks for (or None)."""
     if workspace is None:
@@ -607,7 +611,7 @@ def _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out):
     q, k, v, o = Q.stride(), K.stride(), V.stride(), out.stride()
     if q[2] != 1 or k[2] != 1 or v[2] != 1 or o[2] != 1:
         raise ValueError("the head dimension must be contiguous")
-    if 0 in q or 0 in k or 0 in v or 0 in o:
+    if (0 in q or 0 in k or 0 in v or 0 in o) and _expanded((qs, q), (ks, k), (ks, v), (qs, o)):
         raise ValueError("expanded tensors (strides of 0) are not supported")
     code = _KINDS.get(Q.dtype)
     if code is None:
@@ -659,7 +663,7 @@ def _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out):
     sq, so, sp, sk = q.stride(), out.stride(), K_prefix.stride(), K.stride()
     if sp != V_prefix.stride() or sk != V.stride():
         raise ValueError("K and V must have the same strides")
-    if 0 in sq or 0 in so or 0 in sp or 0 in sk:
+    if (0 in sq or 0 in so or 0 in sp or 0 in sk) and _expanded((qs, sq), (qs, so), (ps, sp), (ks, sk)):
         raise ValueError("expanded tensors (strides of 0) are not supported")
     # a dimension of one element may have any stride
     if sp[2] != 1 or sk[3] != 1 or (room > 1 and sp[1] != D) or (most > 1 and sk[2] != D):

@@ -70,9 +70,9 @@ int checked(const b200p_packed_args* args, b200p_packed_args* out) {
     const long long D = a.D;
     auto fill = [&](long long& token, long long& head, long long heads) { if (token == 0 && head == 0) { token = heads * D; head = D; } };
     fill(a.q_token, a.q_head, a.nQHeads); fill(a.k_token, a.k_head, a.nKVHeads); fill(a.v_token, a.v_head, a.nKVHeads); fill(a.o_token, a.o_head, a.nQHeads);
-    // the stride of a dimension of one element says nothing
-    if (a.total_q == 1) a.q_token = a.o_token = a.nQHeads * D;
-    if (a.total_k == 1) a.k_token = a.v_token = a.nKVHeads * D;
+    // the stride of a dimension of one element, or none, says nothing
+    if (a.total_q <= 1) a.q_token = a.o_token = a.nQHeads * D;
+    if (a.total_k <= 1) a.k_token = a.v_token = a.nKVHeads * D;
     if (a.nQHeads == 1) a.q_head = a.o_head = D;
     if (a.nKVHeads == 1) a.k_head = a.v_head = D;
     for (long long s : {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head, a.o_token, a.o_head}) if (s <= 0 || s % 8 != 0) return B200P_E_ALIGN;

@@ -251,6 +251,9 @@ def test_nothing_to_do(b200p, torch_cuda, splits):
     torch = torch_cuda
     Q, K, V, qo, ko = make(torch, [0], [0], 4, 2, 64, torch.bfloat16)
     assert b200p.prefill_packed(Q, K, V, qo).shape == (0, 4, 64)
+    Q, K, V, qo, ko = make(torch, [5], [0], 1, 1, 64, torch.bfloat16)         # no keys: an empty tensor's strides may be anything
+    for empty in (K, K.as_strided((0, 1, 64), (0, 0, 1)), K.as_strided((0, 1, 64), (7, 3, 1))):
+        assert (b200p.prefill_packed(Q, empty, empty, qo, ko) == 0).all()
     Q, K, V, qo, ko = make(torch, [5], [5], 4, 2, 64, torch.bfloat16)
     out = torch.full_like(Q, 7.0)
     assert (b200p.prefill_packed(Q, K, V, torch.zeros(1, dtype=torch.int32, device="cuda"), out=out) == 7.0).all()
