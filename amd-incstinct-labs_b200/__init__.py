@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libb200p.so")
@@ -541,6 +542,10 @@ class SharedArgs(C.Structure):
         (n, _ll) for n in ("prefix_head", "own_head", "own_batch", "q_batch", "o_batch")]
 
 
+# the same structures as bytes: a small call spends less on these than on a ctypes object's fields
+_PACKED_BYTES, _SHARED_BYTES, _LOGITS_BYTES = struct.Struct("@8if8q"), struct.Struct("@7if5q"), struct.Struct("@7i2q11P")
+
+
 class LogitsArgs(C.Structure):
     """struct b200p_logits_args (include/b200p.h)."""
     _fields_ = [(n, _i) for n in ("dtype", "rows", "vocab", "prompt_max", "tokens_max", "bias_n", "n_masks")] + [
@@ -569,12 +574,13 @@ def _together(first, tensors, ints=()):
     for t in tensors:
         if t.get_device() != device:
             raise ValueError("all tensors of a call must be on one CUDA device")
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise ValueError("a call's Q, K, V and output, or logits and output, must have one type")
+    int32 = torch.int32
     for t in ints:
         if t.get_device() != device:
             raise ValueError("all tensors of a call must be on one CUDA device")
-        if t.dtype != torch.int32 or not t.is_contiguous():
+        if t.dtype is not int32 or not t.is_contiguous():
             raise ValueError("offsets, lengths and ids must be contiguous int32 tensors")
     return device
 
@@ -594,7 +600,7 @@ def _expanded(*shapes_and_strides):
 def _scratch(workspace, size, a, like, device):
     """The caller's workspace, or one made for this call, of the size that the library asks for (or None)."""
     if workspace is None:
-        n = _on(device, size, C.byref(a))
+        n = _on(device, size, a)
         return like.new_empty(n, dtype=_torch.uint8) if n else None
     if workspace.get_device() != device or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on the other tensors' device")
@@ -602,7 +608,8 @@ def _scratch(workspace, size, a, like, device):
 
 
 def _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out):
-    torch = _torch or _bind()
+    if _torch is None:
+        _bind()
     qs, ks, shape = Q.shape, K.shape, q_offsets.shape
     if len(qs) != 3 or len(ks) != 3 or ks != V.shape or out.shape != qs or ks[2] != qs[2]:
         raise ValueError("Q and out are [tokens, heads, D], K and V [tokens, kv_heads, D]")
@@ -616,13 +623,13 @@ def _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out):
     code = _KINDS.get(Q.dtype)
     if code is None:
         raise ValueError("Q, K and V must be fp16 or bf16")
-    return PackedArgs(qs[2], qs[1], ks[1], shape[0] - 1, qs[0], ks[0], 1 if causal else 0, code, scale, q[0], q[1], k[0], k[1], v[0], v[1], o[0], o[1])
+    return _PACKED_BYTES.pack(qs[2], qs[1], ks[1], shape[0] - 1, qs[0], ks[0], 1 if causal else 0, code, scale, q[0], q[1], k[0], k[1], v[0], v[1], o[0], o[1])
 
 
 def prefill_packed_workspace(Q, K, V, q_offsets, k_offsets=None, causal: bool = True):
     """Scratch tensor for prefill_packed with tensors of these shapes (it may be empty)."""
     a = _packed_args(Q, K, V, q_offsets, q_offsets if k_offsets is None else k_offsets, causal, 0.0, Q)
-    return Q.new_empty(_on(_together(Q, (K, V)), lib().b200p_attn_prefill_packed_workspace_bytes, C.byref(a)), dtype=_torch.uint8)
+    return Q.new_empty(_on(_together(Q, (K, V)), lib().b200p_attn_prefill_packed_workspace_bytes, a), dtype=_torch.uint8)
 
 
 def prefill_packed(Q, K, V, q_offsets, k_offsets=None, causal: bool = True, scale: float = 0.0, out=None, workspace=None):
@@ -638,14 +645,18 @@ def prefill_packed(Q, K, V, q_offsets, k_offsets=None, causal: bool = True, scal
     device = _together(Q, (K, V, out), (q_offsets, k_offsets))
     a = _packed_args(Q, K, V, q_offsets, k_offsets, causal, scale, out)
     L = lib()
-    ws = _scratch(workspace, L.b200p_attn_prefill_packed_workspace_bytes, a, Q, device)
-    _check(_on(device, L.b200p_attn_prefill_packed, Q.data_ptr(), K.data_ptr(), V.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), out.data_ptr(), C.byref(a),
-               None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(Q)), "attn_prefill_packed")
+    call = (Q.data_ptr(), K.data_ptr(), V.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), out.data_ptr(), a)
+    status = -7 if workspace is not None else _on(device, L.b200p_attn_prefill_packed, *call, None, 0, _stream(Q))      # most calls need none
+    if status == -7:                                              # refused ahead of any launch
+        ws = _scratch(workspace, L.b200p_attn_prefill_packed_workspace_bytes, a, Q, device)
+        status = _on(device, L.b200p_attn_prefill_packed, *call, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(Q))
+    _check(status, "attn_prefill_packed")
     return out
 
 
 def _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out):
-    torch = _torch or _bind()
+    if _torch is None:
+        _bind()
     qs, ps, ks = q.shape, K_prefix.shape, K.shape
     if len(qs) != 3 or len(ps) != 3 or len(ks) != 4 or ps != V_prefix.shape or ks != V.shape or out.shape != qs:
         raise ValueError("q and out are [batch, heads, D], the prefix [kv_heads, keys, D], K and V [batch, kv_heads, keys, D]")
@@ -670,14 +681,14 @@ def _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out):
         raise ValueError("the rows of a key head must follow one another")
     if sq[2] != 1 or so[2] != 1 or (heads > 1 and (sq[1] != D or so[1] != D)):
         raise ValueError("the heads of q and of out must follow one another")
-    return SharedArgs(D, heads, kv, batch, n, most, code, scale, sp[0] if kv > 1 else room * D, sk[1] if kv > 1 else most * D,
+    return _SHARED_BYTES.pack(D, heads, kv, batch, n, most, code, scale, sp[0] if kv > 1 else room * D, sk[1] if kv > 1 else most * D,
                       sk[0] if batch > 1 else kv * (sk[1] if kv > 1 else most * D), sq[0] if batch > 1 else heads * D, so[0] if batch > 1 else heads * D)
 
 
 def decode_shared_workspace(q, K_prefix, K, prefix_len=None):
     """Scratch tensor for decode_shared with tensors of these shapes (it may be empty)."""
     a = _shared_args(q, K_prefix, K_prefix, K, K, prefix_len, 0.0, q)
-    return q.new_empty(_on(_together(q, (K_prefix, K)), lib().b200p_attn_decode_shared_workspace_bytes, C.byref(a)), dtype=_torch.uint8)
+    return q.new_empty(_on(_together(q, (K_prefix, K)), lib().b200p_attn_decode_shared_workspace_bytes, a), dtype=_torch.uint8)
 
 
 def decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len=None, scale: float = 0.0, out=None, workspace=None):
@@ -694,7 +705,7 @@ def decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len=None, scale: 
     L = lib()
     ws = _scratch(workspace, L.b200p_attn_decode_shared_workspace_bytes, a, q, device)
     _check(_on(device, L.b200p_attn_decode_shared, q.data_ptr(), K_prefix.data_ptr(), V_prefix.data_ptr(), K.data_ptr(), V.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-               C.byref(a), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(q)), "attn_decode_shared")
+               a, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(q)), "attn_decode_shared")
     return out
 
 
@@ -717,7 +728,7 @@ def adjust_logits(logits, prompt=None, prompt_lengths=None, tokens=None, token_l
         raise ValueError("logits must be fp32, fp16 or bf16")
     device = _together(logits, (out,), [t for t in (prompt, prompt_lengths, tokens, token_lengths, bias_ids, mask, mask_rows) if t is not None])
     for t in (repetition, presence, frequency, bias_values):
-        if t is not None and (t.get_device() != device or t.dtype != torch.float32 or not t.is_contiguous()):
+        if t is not None and (t.get_device() != device or t.dtype is not torch.float32 or not t.is_contiguous()):
             raise ValueError("penalties and bias values must be contiguous fp32 tensors on the logits' device")
     for t in (prompt_lengths, token_lengths, repetition, presence, frequency, mask_rows):
         if t is not None and t.shape != (R,):
@@ -738,14 +749,14 @@ def adjust_logits(logits, prompt=None, prompt_lengths=None, tokens=None, token_l
         return out
 
     def ptr(t):
-        return None if t is None else t.data_ptr() or None        # an empty tensor has no address
+        return 0 if t is None else t.data_ptr()                   # 0 as well for an empty tensor
 
     def width(t):
         return 0 if t is None else t.shape[1]
-    a = LogitsArgs(code, R, V, width(prompt), width(tokens), width(bias_ids), 0 if mask is None else mask.shape[0], si[0] if R > 1 else V, so[0] if R > 1 else V,
+    a = _LOGITS_BYTES.pack(code, R, V, width(prompt), width(tokens), width(bias_ids), 0 if mask is None else mask.shape[0], si[0] if R > 1 else V, so[0] if R > 1 else V,
                    ptr(prompt), ptr(prompt_lengths), ptr(tokens), ptr(token_lengths), ptr(repetition), ptr(presence), ptr(frequency), ptr(bias_ids), ptr(bias_values),
                    ptr(mask), ptr(mask_rows))
-    _check(_on(device, lib().b200p_logits_adjust, logits.data_ptr(), out.data_ptr(), C.byref(a), _stream(logits)), "logits_adjust")
+    _check(_on(device, lib().b200p_logits_adjust, logits.data_ptr(), out.data_ptr(), a, _stream(logits)), "logits_adjust")
     return out
 
 

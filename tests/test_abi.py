@@ -47,6 +47,14 @@ def test_argument_errors_come_before_any_launch(b200p):
     assert b200p.set_tuning("no_such_knob", 1) == -2 ** 31
 
 
+def test_packed_bytes_are_the_structures(b200p):
+    for as_bytes, struct in ((b200p._PACKED_BYTES, b200p.PackedArgs), (b200p._SHARED_BYTES, b200p.SharedArgs), (b200p._LOGITS_BYTES, b200p.LogitsArgs)):
+        assert as_bytes.size == C.sizeof(struct)
+        values = list(range(1, len(struct._fields_) + 1))
+        a = struct.from_buffer_copy(as_bytes.pack(*values))
+        assert [getattr(a, n) for n, _ in struct._fields_] == values
+
+
 def test_no_cpu_fallback(b200p):
     import torch
     x = torch.zeros(64)
