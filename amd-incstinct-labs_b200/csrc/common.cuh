@@ -43,7 +43,7 @@ enum Knob {
     KNOB_DELTA_TENSOR,          // 0: blocks of 16-bit sessions without tensor cores as well
     KNOB_SKINNY_CLUSTER,        // 1..8: CTAs that share K in skinny_tc_kernel, where K has as many blocks of 64 columns (0: chosen from the shape)
     KNOB_PACKED_SPLITS,         // packed prefill: how often the keys are split (0: chosen)
-    KNOB_SHARED_PREFIX,         // decode behind a shared prefix: 1 the prefix read per sequence, 2 once by tcgen05 tiles (0: chosen)
+    KNOB_SHARED_PREFIX,         // decode behind a shared prefix: 1 the prefix read per sequence, 2 once by tcgen05 tiles, 3 the same without a launch for the merge (0: chosen)
     KNOB_SHARED_SPLITS,         // the same, form 2: how often the prefix's keys are split (0: chosen)
     KNOB_COUNT
 };

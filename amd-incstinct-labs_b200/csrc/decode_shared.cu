@@ -4,21 +4,21 @@
 //
 // Softmax over both parts is the merge of what each part gives (m: maximum, l: sum, O: weighted sum of values):
 //   m = max m_i;  l = sum l_i 2^(m_i - m);  O = sum O_i 2^(m_i - m) / l.
-// Three launches:
+// Two or three launches:
 //  1. the prefix, for the whole batch: the query rows of a key head are ONE matrix of batch * group rows, so this is the tcgen05
 //     prefill kernel (packed.cuh) over one "sequence" of `batch` tokens without a mask, its keys split so that all SMs have work;
 //     (m, l, O) of every split go to the workspace in fp32.  Each tile of the prefix is read once per 256 rows.
 //  2. the sequences' own keys (own_kernel): HBM-bound, every byte of the caches is read once.  A programmatic dependent that
 //     waits for nothing: its CTAs run wherever the first launch leaves room.
-//  3. the merge (merge_kernel, packed_launch.cuh).
+//  3. the merge (merge_kernel, packed_launch.cuh); or the second launch waits for the first and merges itself (plan_shared).
 // A prefix that is small for its batch is cheaper read per sequence (from L2), by own_kernel, which then is the only launch.
 //
-// Measured, calls replayed from a graph, 32 / 8 heads of 128 unless said otherwise: 4 sequences, 512 keys in front, up to 32 of their own 6.2 us (one
-// launch); 32, 2000, up to 512, fp16, 17 us; 48 with 32 / 4 heads of 64, 5000, up to 1000, 18.7; 256, 32768, up to 256, 143 to 160 (960 TFLOP/s and
-// more, the tiles at the prefill kernel's rate).  What bounds the middle ones is latency: three dependent launches, of which the tiles' takes 4.5 us
-// for its barriers, Q, first keys and way out and 1.35 a key tile, the own keys' 10 from start to end, the merge 3.
+// Measured, calls replayed from a graph, 32 / 8 heads of 128 unless said otherwise: 4 sequences, 512 keys in front, up to 32 of their own 6.5 us (one
+// launch); 32, 2000, up to 512, fp16, 16.6; 48 with 32 / 4 heads of 64, 5000, up to 1000, 19.2; 256, 32768, up to 256, 141 to 160 (980 TFLOP/s and
+// more, the tiles at the prefill kernel's rate).  What bounds the middle ones is latency: dependent launches, of which the tiles' takes 4.5 us
+// for its barriers, Q, first keys and way out and 1.35 a key tile, the own keys' 10 from start to end, the merge 2 to 3.
 // (Not kept: the prefix by mma.sync warps that share their keys through L1, 4 warps of 16 rows each, never clearly faster than the tiles, 220 against
-// 55 us for 34 sequences behind 25299 keys; the merge inside the second launch, whose CTAs then hold their SMs until the prefix is done, 27 against 17 us.)
+// 55 us for 34 sequences behind 25299 keys.)
 // ---------------------------------------------------------------------------
 #include "packed_launch.cuh"
 
@@ -29,6 +29,7 @@ constexpr int kOwnWarps = 4;
 constexpr int kOwnThreads = kOwnWarps * 32;
 constexpr int kKeyBlock = 16;                    // keys of a warp's step
 constexpr int kMostOwnCluster = 8;
+constexpr int kMostJoined = 32;                  // splits that own_kernel merges itself: a lane each
 constexpr int kMostSplits = kMostParts - kMostOwnCluster;        // of the prefix: one for each SM, for a single key head
 
 struct OwnParams {
@@ -41,6 +42,7 @@ struct OwnParams {
     float scale_log2;
     int apart;                                   // 1: results go to the workspace, as parts `first_part` + the CTA's place in its unit
     int first_part;
+    int joined;                                  // splits of the prefix that this launch waits for and merges itself
     float *part_o, *part_ml;                     // [part][batch][nQH][D], not divided; [..][2]: maximum in log2 units, sum
 };
 
@@ -62,20 +64,6 @@ __device__ __forceinline__ float4 load_cluster_f32x4(uint32_t smem, uint32_t cta
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(cta));
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
-}
-
-// 2^(m_i - m) of this lane's part, m the maximum over the warp, and 1 / sum of 2^(m_i - m) l_i.  A sum of 0 is a part without keys, whose O
-// means nothing.
-__device__ __forceinline__ float part_weight(float2 ml, float& inv) {
-    float most = ml.x;
-    #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    const float f = ml.y == 0.f ? 0.f : weight_of(ml.x, most);
-    float sum = f * ml.y;
-    #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    inv = 1.f / sum;
-    return f;
 }
 
 // Up to 8 * NT query rows against blocks of 16 keys by one warp.  A step is S^T = K Q^T and O^T += V^T P^T with mma.sync m16n8k16: keys,
@@ -212,7 +200,7 @@ own_kernel(const OwnParams p) {
     __shared__ __align__(16) float s_o[kOwnWarps][R][D + 4];
     __shared__ float s_ml[kOwnWarps][R][2];
     __shared__ float s_sum_ml[R][2];                      // the CTA's, for the cluster; its O takes the first warp's place
-    __shared__ float s_w[R][kMostOwnCluster];
+    __shared__ float s_w[R][kMostOwnCluster + kMostJoined];
     griddep_launch_dependents();                          // the merge may get ready
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int ctas = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y / p.row_groups, r0 = (blockIdx.y % p.row_groups) * R, b = blockIdx.z;
@@ -278,16 +266,26 @@ own_kernel(const OwnParams p) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    // every part's weight in the sum, 2^(m_i - m) / l: a warp per row
+    if (p.joined) griddep_wait();                         // the prefix's splits are there
+    // every part's weight in the sum, 2^(m_i - m) / l, a warp per row: this unit's warps or CTAs, the prefix's splits
     const int parts = ctas > 1 ? ctas : kOwnWarps;
+    const size_t part0 = size_t(b) * nQH + head0, next = size_t(p.batch) * nQH;
     for (int row = warp; row < rows; row += kOwnWarps) {
-        float2 ml = make_float2(-INFINITY, 0.f);
+        float2 ml = make_float2(-INFINITY, 0.f), pml = ml;
+        if (lane < p.joined) pml = __ldcg(reinterpret_cast<const float2*>(&p.part_ml[2 * (part0 + row + lane * next)]));
         if (lane < parts)
             ml = ctas > 1 ? make_float2(load_cluster_f32(dme::smem_addr(&s_sum_ml[row][0]), lane), load_cluster_f32(dme::smem_addr(&s_sum_ml[row][1]), lane))
                           : make_float2(s_ml[lane][row][0], s_ml[lane][row][1]);
-        float inv;
-        const float f = part_weight(ml, inv);
-        if (lane < parts) s_w[row][lane] = p.prefix_here + own > 0 ? f * inv : 0.f;
+        float most = fmaxf(ml.x, pml.x);
+        #pragma unroll
+        for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        const float f = ml.y == 0.f ? 0.f : weight_of(ml.x, most), g = pml.y <= 0.f ? 0.f : weight_of(pml.x, most);     // no key, or nothing but scores of -inf
+        float sum = f * ml.y + (g == 0.f ? 0.f : g * pml.y);
+        #pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float inv = p.joined + p.prefix_here + own > 0 ? 1.f / sum : 0.f;
+        if (lane < parts) s_w[row][lane] = f * inv;
+        if (lane < p.joined) s_w[row][kMostOwnCluster + lane] = g == 0.f && inv < INFINITY ? 0.f : g * inv;
     }
     __syncthreads();
     // four columns per thread
@@ -295,6 +293,15 @@ own_kernel(const OwnParams p) {
     for (int i = rank * share + threadIdx.x; i < last; i += kOwnThreads) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
         float x[4] = {0.f, 0.f, 0.f, 0.f};
+        const float* at = p.part_o + (part0 + row) * D + d;
+        #pragma unroll 8
+        for (int k = 0; k < p.joined; ++k) {
+            const float f = s_w[row][kMostOwnCluster + k];
+            float v[4];
+            load_part<4>(at + k * next * D, v);
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) if (f != 0.f) x[e] += f * v[e];           // where there was no key nothing was stored
+        }
         for (int k = 0; k < parts; ++k) {
             const float4 v = ctas > 1 ? load_cluster_f32x4(dme::smem_addr(&s_o[0][row][d]), k) : *reinterpret_cast<const float4*>(&s_o[k][row][d]);
             const float f = s_w[row][k];
@@ -312,16 +319,17 @@ own_kernel(const OwnParams p) {
 // How a call is run.
 struct SharedPlan {
     int splits, span;            // the prefix in a launch of its own: its splits, tiles of an item; 0: none, own_kernel reads the prefix
+    bool joined;                 // own_kernel waits for the splits and merges them, no third launch
     int cluster, rows;           // CTAs and query rows (8 or 16) of a unit of own_kernel
     size_t off_ml, ws_bytes;
 };
 
 // Times in microseconds, from sizes alone, as they were measured over the range (sequences 2 to 256, prefixes of 100 to 32768 keys, 1 to 8
-// key heads of 64 and 128, own caches up to 2000; a choice is within 15 % of the best one tried).  The sequences' own lengths are not known
+// key heads of 64 and 128, own caches up to 2000; of 145 drawn calls one in ten was more than 5 % above the best form tried, none 25 %).  The sequences' own lengths are not known
 // here: a little over half the caches' room.
-//  * own_kernel alone: 4.5, and what it reads (the prefix for every sequence, from L2) at 7 TB/s or a warp's blocks of 16 keys at 0.6 each.
-//    (32 / 8 heads of 128, 4 sequences, 512 keys in front: 6.2 against 8.0 with the prefix apart; 32 sequences, 2000 keys: 41 against 17.)
-//  * the prefix apart: 5.5 for the launches and the merge; an item of the tcgen05 kernel takes 4.5 and 1.35 per key tile, 2.05 with two
+//  * own_kernel alone: 4.5, and what it reads (the prefix for every sequence, from L2) at 7 TB/s or a warp's blocks of 16 keys at 0.8 each.
+//    (32 / 8 heads of 128, 4 sequences, 512 keys in front: 6.5 against 9.0 with the prefix apart; 32 sequences, 2000 keys: 41 against 17.)
+//  * the prefix apart: 5 for the launches and the merge; an item of the tcgen05 kernel takes 4.5 and 1.35 per key tile, 2.05 with two
 //    query tiles; the own keys are read at 44 GB/s per SM, by the SMs that have no item and, once the items are done, by all; the parts are
 //    written and read again.  (32 sequences, 2000 + up to 512 keys: 4 splits on 32 SMs 16.9, 8 on 64 18.9, 2 on 16 22.6.)
 SharedPlan plan_shared(const b200p_shared_args& a) {
@@ -338,7 +346,7 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
     if (a.prefix_len == 0) return pl;
     const double own_keys = 0.55 * a.max_own, key_bytes = 4.0 * a.D * a.nKVHeads;
     const double here_bytes = a.batch * (a.prefix_len + own_keys) * key_bytes;
-    const double here_walk = 0.6 * ((a.prefix_len + own_keys) / (kKeyBlock * kOwnWarps * pl.cluster) + 1);
+    const double here_walk = 0.8 * ((a.prefix_len + own_keys) / (kKeyBlock * kOwnWarps * pl.cluster) + 1);
     const double here = 4.5 + (here_bytes / 7e6 > here_walk ? here_bytes / 7e6 : here_walk);
     const double own_work = a.batch * own_keys * key_bytes / 44e3;              // of one SM
     const int tokens = kBM / group, tiles = (a.batch + tokens - 1) / tokens, steps = (a.prefix_len + kBN - 1) / kBN, fixed = tuning(KNOB_SHARED_SPLITS, 0);
@@ -360,10 +368,21 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
         }
     }
     const int forced = tuning(KNOB_SHARED_PREFIX, 0);
-    if (splits > 0 && forced != 1 && (forced == 2 || 5.5 + best < here)) {
+    if (splits > 0 && forced != 1 && (forced >= 2 || 5 + best < here)) {
         pl.splits = splits; pl.span = span;
         pl.cluster = cluster_for(a.max_own);
-        const size_t all = size_t(pl.splits + pl.cluster) * a.batch * a.nQHeads;
+        // Where all of own_kernel's CTAs have room beside the items and there are few parts to add up for each, it may wait for them
+        // and merge, which saves a launch (99 sequences, 2423 + up to 441 keys, 6 / 2 heads of 64, 14.9 -> 13.5 us; 145, 2984 + up to 306, 2 / 1,
+        // 11.5 -> 9.9).  CTAs that wait where there is no room hold the SMs that others could begin on (48 of 32 / 4 heads of 64, 5000 + up to 1000,
+        // 19.2 -> 26.4; 256, 32768 + up to 256, 32 / 8 of 128, 141 -> 157); short caches of heads of 64 are read soon enough all the same (103,
+        // 4127 + up to 140, 16 / 4, 18.4 -> 16.1).  Many parts are quicker in merge_kernel's many warps (2 sequences, 14997 + up to 191, 16 / 4 of 128, 15.2 against 16.8).
+        const long long items = (long long)((tiles + span - 1) / span) * a.nKVHeads * splits;
+        const long long room = (a.D == 64 && a.max_own <= 160 ? sms : sms - items) * (pl.rows == 8 ? 4 : a.D == 64 ? 3 : 2);
+        int c = pl.cluster;
+        while (c > 1 && units * c > room && a.max_own <= 300 * c) c /= 2;
+        pl.joined = splits <= kMostJoined && (forced == 3 || (forced != 2 && units * c <= room && group * splits * a.D <= 6500));
+        if (pl.joined) pl.cluster = c;
+        const size_t all = size_t(pl.splits + (pl.joined ? 0 : pl.cluster)) * a.batch * a.nQHeads;
         pl.off_ml = (all * a.D * 4 + 255) / 256 * 256;
         pl.ws_bytes = pl.off_ml + (all * 8 + 255) / 256 * 256;
     }
@@ -415,9 +434,9 @@ int launch(const void* q, const void* Kp, const void* Vp, const void* K, const v
     w.batch = a.batch; w.nKVH = a.nKVHeads; w.group = group; w.max_own = a.max_own; w.row_groups = (group + pl.rows - 1) / pl.rows;
     w.prefix_here = apart ? 0 : a.prefix_len;
     w.prefix_head = a.prefix_head; w.own_head = a.own_head; w.own_batch = a.own_batch; w.q_batch = a.q_batch; w.o_batch = a.o_batch;
-    w.scale_log2 = scale_log2; w.apart = apart; w.first_part = pl.splits; w.part_o = part_o; w.part_ml = part_ml;
+    w.scale_log2 = scale_log2; w.apart = apart && !pl.joined; w.first_part = pl.splits; w.joined = pl.joined ? pl.splits : 0; w.part_o = part_o; w.part_ml = part_ml;
     if (int e = pl.rows == 8 ? launch_own<T, D, 1>(w, pl.cluster, apart, st) : launch_own<T, D, 2>(w, pl.cluster, apart, st)) return e;
-    if (!apart) return B200P_OK;
+    if (!apart || pl.joined) return B200P_OK;
     return launch_merge<T, D>(part_o, part_ml, pl.splits + pl.cluster, a.batch, a.nQHeads, o, a.o_batch, D, nullptr, nullptr, st);
 }
 

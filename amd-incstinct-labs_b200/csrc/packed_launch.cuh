@@ -52,26 +52,36 @@ int launch_packed(PackedParams p, int dtype, cudaStream_t st) {
 // ---- parts of rows (the splits' results) into the rows' results ------------------------------------------
 constexpr int kMostParts = 160;
 constexpr int kMergeWarps = 4;
+constexpr int kFewParts = 12;
 
 __device__ __forceinline__ float weight_of(float m, float most) { return exp2f(m - (most == -INFINITY ? 0.f : most)); }
 
-// Row r = token * nQH + head from part_o[s][r][D] and part_ml[s][r]: a warp per row.  m = max m_s, O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s;
+// From L2.  Volatile: a load must not move behind the test whether its part counts, or each waits for the one before it.
+template <int E> __device__ __forceinline__ void load_part(const float* at, float (&v)[E]) {
+    static_assert(E == 2 || E == 4);
+    if constexpr (E == 4) asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "l"(at) : "memory");
+    else asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "l"(at) : "memory");
+}
+
+// Row r = token * nQH + head from part_o[s][r][D] and part_ml[s][r].  m = max m_s, O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s;
 // parts without a key do not count, a row without any gives zeros.  first, last: device words with the first row to be written and the one
-// behind the last, in tokens, or null.
-template <typename T, int D>
+// behind the last, in tokens, or null.  A warp per row; of many parts, a row's four warps take every fourth (86 parts of 32 rows of 64, the whole
+// call: 18.8 -> 10.4 us; a part's load is L2 latency, and few rows have few warps to hide it).
+template <typename T, int D, bool MANY>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int parts, int tokens, int nQH, T* __restrict__ o, long long o_token, long long o_head,
              const int* first, const int* last) {
-    constexpr int E = D / 32;
-    __shared__ float s_f[kMergeWarps][kMostParts];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x * kMergeWarps + warp, rows = tokens * nQH, token = row / nQH;
+    constexpr int E = D / 32, P = ((MANY ? kMostParts : kFewParts) + 31) / 32, STEP = MANY ? kMergeWarps : 1;
+    __shared__ float s_f[kMergeWarps][32 * P];
+    __shared__ float s_x[MANY ? kMergeWarps : 1][MANY ? D : 1];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = MANY ? blockIdx.x : blockIdx.x * kMergeWarps + warp, rows = tokens * nQH, token = row / nQH;
     griddep_wait();
     if (row >= rows || (first && (token < *first || token >= *last))) return;
-    float2 ml[kMostParts / 32];
+    float2 ml[P];
     float most = -INFINITY;
     bool some = false;
     #pragma unroll
-    for (int k = 0; k < kMostParts / 32; ++k) {
+    for (int k = 0; k < P; ++k) {
         const int s = 32 * k + lane;
         ml[k] = s < parts ? __ldcg(reinterpret_cast<const float2*>(&part_ml[2 * (size_t(s) * rows + row)])) : make_float2(-INFINITY, kNoKey);
         most = fmaxf(most, ml[k].x);
@@ -82,7 +92,7 @@ merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml
     some = __any_sync(0xffffffffu, some);
     float sum = 0.f;
     #pragma unroll
-    for (int k = 0; k < kMostParts / 32; ++k) {
+    for (int k = 0; k < P; ++k) {
         const float f = ml[k].y <= 0.f ? 0.f : weight_of(ml[k].x, most);        // no key, or nothing but scores of -inf
         sum += f == 0.f ? 0.f : f * ml[k].y;
         s_f[warp][32 * k + lane] = f;
@@ -92,14 +102,22 @@ merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml
     __syncwarp();
     float x[E] = {};
     #pragma unroll 8
-    for (int s = 0; s < parts; ++s) {
+    for (int s = MANY ? warp : 0; s < parts; s += STEP) {
         float v[E];
-        const float* at = part_o + (size_t(s) * rows + row) * D + lane * E;
-        if constexpr (E == 4) { const float4 w = __ldcg(reinterpret_cast<const float4*>(at)); v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w; }
-        else { const float2 w = __ldcg(reinterpret_cast<const float2*>(at)); v[0] = w.x; v[1] = w.y; }
+        load_part<E>(part_o + (size_t(s) * rows + row) * D + lane * E, v);
         const float f = s_f[warp][s];
         #pragma unroll
-        for (int e = 0; e < E; ++e) if (f != 0.f) x[e] += f * v[e];
+        for (int e = 0; e < E; ++e) if (f != 0.f) x[e] += f * v[e];             // where there was no key nothing was stored
+    }
+    if constexpr (MANY) {
+        #pragma unroll
+        for (int e = 0; e < E; ++e) s_x[warp][lane * E + e] = x[e];
+        __syncthreads();
+        if (warp > 0) return;
+        #pragma unroll
+        for (int k = 1; k < kMergeWarps; ++k)
+            #pragma unroll
+            for (int e = 0; e < E; ++e) x[e] += s_x[k][lane * E + e];
     }
     const float inv = some ? 1.f / sum : 0.f;               // nothing but scores of -inf: 0 / 0
     T* y = o + token * o_token + (row - token * nQH) * o_head + lane * E;
@@ -124,8 +142,10 @@ int launch_after(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A.
 template <typename T, int D>
 int launch_merge(const float* part_o, const float* part_ml, int parts, int tokens, int nQH, void* o, long long o_token, long long o_head, const int* first, const int* last,
                  cudaStream_t st) {
-    const long long ctas = ((long long)tokens * nQH + kMergeWarps - 1) / kMergeWarps;
-    return launch_after(merge_kernel<T, D>, dim3(unsigned(ctas)), kMergeWarps * 32, st, part_o, part_ml, parts, tokens, nQH, static_cast<T*>(o), o_token, o_head, first, last);
+    const long long rows = (long long)tokens * nQH, ctas = (rows + kMergeWarps - 1) / kMergeWarps;
+    if (parts <= kFewParts)
+        return launch_after(merge_kernel<T, D, false>, dim3(unsigned(ctas)), kMergeWarps * 32, st, part_o, part_ml, parts, tokens, nQH, static_cast<T*>(o), o_token, o_head, first, last);
+    return launch_after(merge_kernel<T, D, true>, dim3(unsigned(rows)), kMergeWarps * 32, st, part_o, part_ml, parts, tokens, nQH, static_cast<T*>(o), o_token, o_head, first, last);
 }
 
 } // namespace b200p

@@ -34,7 +34,7 @@ def test_prefix_and_own_keys(b200p, torch_cuda, batch, heads, kv, prefix, own, D
 
 
 # every way to run a call, whatever the sizes would choose: the prefix per sequence, or once, in few and in many splits
-@pytest.mark.parametrize("form,splits", [(1, -1), (2, -1), (2, 1), (2, 3), (2, 1000)])
+@pytest.mark.parametrize("form,splits", [(1, -1), (2, -1), (2, 1), (2, 3), (2, 1000), (3, -1), (3, 1), (3, 3), (3, 30)])
 @pytest.mark.parametrize("batch,heads,kv,D,prefix,own", [(1, 4, 4, 128, 1, 5), (3, 6, 2, 64, 257, 40), (40, 8, 1, 128, 1000, 200), (9, 40, 8, 64, 700, 33), (150, 4, 2, 128, 300, 100),
                                                          (2, 20, 1, 128, 513, 600)])
 def test_every_form(b200p, torch_cuda, batch, heads, kv, D, prefix, own, form, splits):
