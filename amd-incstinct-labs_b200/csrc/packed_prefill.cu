@@ -14,11 +14,13 @@
 namespace b200p {
 namespace {
 
-// In how many splits the keys are taken, for few query tiles with many keys (a few new tokens on a long cache): a tile takes 1.35 us per
-// 128 keys, one after the other; the parts' way through the workspace and the merge take 4 us.  A split has two key tiles at least, going by
-// the mean, and there are no more than SMs: a second round of items costs what it was to save.  (Without and with, 32 / 8 heads of 128:
-// 16 tokens on 8000 keys 101 and 17.5 us; 8 single tokens on 8000 keys 101 and 60; 64 tokens, 1024 keys, 19.1 and 13.6; 300 tokens, 300 keys, 10.3 and, with 2 splits, 11.4: under 1024
-// keys none.)
+// In how many splits the keys are taken: for few query tiles with many keys (a few new tokens on a long cache), and for a few sequences
+// of which some may be much longer than the others.  The lengths are on the device, so the times, in microseconds, go by the means: an
+// item takes 3 and 1.35 per 128 keys (2.05 with two query tiles); the last one to end may be of a sequence 1.8 times as long and begins
+// when the others are under way; the merge takes 3, and the parts' way through the workspace.  A split has two key tiles at least.
+// (One and the number chosen, 8 / 2 heads of 128: 39 tokens each of 11 sequences on 3950 keys 81 and 30; 2 texts of 1000 and 5000 tokens, one head, 72 and 28;
+// 32 / 8 heads: 4 times 16 tokens on 1500 keys 32.6 and 18; 300 tokens, 300 keys, 10.3 and, with 2, 11.4: none.  Of 110 drawn calls of 200 keys and
+// more, twice, the mean is 3 and 4 % above the best number of splits tried, the worst case 1.6 times.)
 struct PackedPlan { int splits; size_t off_ml, ws_bytes; };
 PackedPlan plan_packed(const b200p_packed_args& a) {
     PackedPlan pl{1, 0, 0};
@@ -26,13 +28,21 @@ PackedPlan plan_packed(const b200p_packed_args& a) {
     const int sms = sm_count() > 0 ? sm_count() : 148, group = a.nQHeads / a.nKVHeads;
     const int tokens = kBM / group;
     const long long about = a.total_q / tokens + (a.batch + 1) / 2;            // of a key head: every second sequence fills a tile more than its share
-    const long long tiles = (about > a.batch ? about : a.batch) * a.nKVHeads, keys = a.total_k / a.batch;
+    const long long tiles = (about > a.batch ? about : a.batch) * a.nKVHeads, most_tiles = packed_tiles(a.total_q, a.batch, tokens, a.nKVHeads);
     const int fixed = tuning(KNOB_PACKED_SPLITS, 0);
+    const double keys = double(a.total_k) / a.batch, new_keys = double(a.total_q) / a.batch;
     if (fixed > 0) pl.splits = fixed < kMostParts ? fixed : kMostParts;
-    else if (keys >= 8 * kBN && 2 * tiles <= sms) {
-        const long long s = sms / tiles, most = (keys + 2 * kBN - 1) / (2 * kBN);
-        pl.splits = int(s < most ? s : most);
-        if (pl.splits > kMostParts) pl.splits = kMostParts;
+    else if (keys > 2 * kBN && tiles <= 2 * sms) {
+        const double mean = (keys - (a.causal ? new_keys / 2 : 0)) / kBN, longest = (a.batch > 1 && 1.8 * keys < a.total_k ? 1.8 * keys : a.total_k) / kBN;
+        double best = 0;
+        for (int s = 1; s <= kMostParts && s <= keys / (2 * kBN) + 1; ++s) {
+            const bool pairs = most_tiles * s > sms && new_keys >= 1.5 * tokens;
+            const double step = pairs ? 2.05 : 1.35, items = double(tiles) * s / (pairs ? 2 : 1);
+            const double last = 4.5 + step * std::ceil(longest / s), all = items * (3 + step * (mean > 0.5 * s ? mean / s : 0.5)) / sms + 0.75 * last;
+            double t = items > sms && all > last ? all : last;
+            if (s > 1) t += 3 + double(s) * a.total_q * a.nQHeads * a.D * 8 / 5e6;
+            if (best == 0 || t < best) { best = t; pl.splits = s; }
+        }
     }
     if (pl.splits > 1) {
         const size_t all = size_t(pl.splits) * a.total_q * a.nQHeads;
