@@ -56,7 +56,9 @@ template <typename T> __device__ __forceinline__ void put(uint4& v, int e, T x) 
 // the row it is stored as one, and loaded as one if `in` lies the same way.
 // HBM-bound without histories: 256 rows of 128000 fp32 logits 40.8 us = 6.4 TB/s, with masks 42.  Histories (2048 + 512 ids a row on average, biases)
 // make it 61: a CTA's two barriers and its trips for ids leave the memory idle, and 16 CTAs of a row look at the same ids.  Segments of 16384 and 32768
-// tokens halve and quarter that and take 66 and 74 us: fewer CTAs an SM to fill each other's waits.  One row of 32000: 3.1 us, launch included.
+// tokens halve and quarter that and take 66 and 74 us: fewer CTAs an SM to fill each other's waits.  Each id
+// looked at by one CTA of a cluster of 8, which counts it in its owner's shared memory, 73 (frequent tokens have one owner); ids by 16-byte loads 63.
+// One row of 32000: 3.1 us, launch included.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4)
 logits_kernel(const LogitsParams p, const T* in, T* out) {

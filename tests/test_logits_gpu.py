@@ -55,6 +55,38 @@ def test_rules(b200p, torch_cuda, rows, vocab, prompt, tokens, bias, masks, kind
     assert torch.equal(other[:, 2:2 + vocab], got) and (other[:, :2] == 7.0).all() and (other[:, vocab + 2:] == 7.0).all()
 
 
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab,prompt,tokens,bias,masks", [
+    (1, 16385, 1024, 0, 0, 0), (2, 20000, 0, 1024, 3, 1), (1, 32000, 1, 1023, 0, 0), (3, 50001, 2000, 500, 8, 2), (2, 65535, 9000, 3000, 1024, 1), (1, 65536, 1100, 0, 2, 1),
+    (2, 65537, 700, 700, 2, 1), (1, 131079, 3000, 9000, 33, 1)])
+def test_long_histories_of_large_vocabularies(b200p, torch_cuda, rows, vocab, prompt, tokens, bias, masks, kind):
+    """Histories longer than the first loads take, several segments; with the ids at the segments' and the vocabulary's ends, and one id many times."""
+    torch = torch_cuda
+    x = request(torch, rows, vocab, prompt, tokens, bias, masks, seed=vocab + prompt)
+    ends = [t for at in range(0, vocab, 8192) for t in range(at - 5, at + 2)] + [vocab - 1, vocab, -1]
+    for name in ("prompt", "tokens"):
+        if name in x:
+            n = min(x[name].shape[1], len(ends))
+            x[name][:, :n] = torch.tensor(ends[:n], dtype=torch.int32, device="cuda")
+            x[name][:, -x[name].shape[1] // 4:] = vocab - 2
+    logits = (4 * torch.randn(rows, vocab, device="cuda")).to(getattr(torch, kind))
+    got = b200p.adjust_logits(logits, **x)
+    want, bound = ref.adjusted(logits, **x)
+    same(torch, got, want, bound)
+    buf = torch.full((rows, vocab + 7), 7.0, device="cuda", dtype=logits.dtype)
+    for at in (1, 3, 6):
+        buf.fill_(7.0)
+        view = buf[:, at:at + vocab]
+        view.copy_(logits)
+        b200p.adjust_logits(view, out=view, **x)
+        assert torch.equal(view, got) and (buf[:, :at] == 7.0).all() and (buf[:, at + vocab:] == 7.0).all()
+    for name in ("prompt_lengths", "token_lengths"):
+        if name in x:
+            x[name].zero_()
+    short = b200p.adjust_logits(logits, **x)
+    same(torch, short, *ref.adjusted(logits, **x))
+
+
 def test_without_rules_the_logits_stay(b200p, torch_cuda):
     torch = torch_cuda
     logits = torch.randn(3, 777, device="cuda")
