@@ -28,10 +28,14 @@ struct RowRules {
     const int* bias_ids; const float* bias_values; int bias_n;
 };
 
+// By selection rather than branches: a thread does its touched tokens one after the other, and a warp takes every branch that one of its
+// lanes takes (48 rows of 50001, bf16: 7.7 us, so 7.4).
 __device__ __forceinline__ float adjusted(float x, unsigned word, int token, const RowRules& r) {
-    if (word & (kInPrompt | kCount)) x = x > 0.f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
+    const float less = __fdiv_rn(x, r.repetition), more = __fmul_rn(x, r.repetition);
+    x = word & (kInPrompt | kCount) ? (x > 0.f ? less : more) : x;
     const unsigned count = word & kCount;
-    if (count) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.frequency, float(count))), r.presence);
+    const float taken = __fsub_rn(__fsub_rn(x, __fmul_rn(r.frequency, float(count))), r.presence);
+    x = count ? taken : x;
     if (word & kBiased) {
         float b = 0.f;
         for (int i = 0; i < r.bias_n; ++i) if (r.bias_ids[i] == token) b = __fadd_rn(b, r.bias_values[i]);
