@@ -14,7 +14,7 @@
 // A prefix that is small for its batch is cheaper read per sequence (from L2), by own_kernel, which then is the only launch.
 //
 // Measured, calls replayed from a graph, 32 / 8 heads of 128 unless said otherwise: 4 sequences, 512 keys in front, up to 32 of their own 6.5 us (one
-// launch); 32, 2000, up to 512, fp16, 16.6; 48 with 32 / 4 heads of 64, 5000, up to 1000, 19.2; 256, 32768, up to 256, 141 to 160 (980 TFLOP/s and
+// launch); 32, 2000, up to 512, fp16, 16.6; 48 with 32 / 4 heads of 64, 5000, up to 1000, 18.7; 256, 32768, up to 256, 141 to 160 (980 TFLOP/s and
 // more, the tiles at the prefill kernel's rate).  What bounds the middle ones is latency: dependent launches, of which the tiles' takes 4.5 us
 // for its barriers, Q, first keys and way out and 1.35 a key tile, the own keys' 10 from start to end, the merge 2 to 3.
 // (Not kept: the prefix by mma.sync warps that share their keys through L1, 4 warps of 16 rows each, never clearly faster than the tiles, 220 against
@@ -325,7 +325,7 @@ struct SharedPlan {
 };
 
 // Times in microseconds, from sizes alone, as they were measured over the range (sequences 2 to 256, prefixes of 100 to 32768 keys, 1 to 8
-// key heads of 64 and 128, own caches up to 2000; of 145 drawn calls one in ten was more than 5 % above the best form tried, none 25 %).  The sequences' own lengths are not known
+// key heads of 64 and 128, own caches up to 2000; of 460 drawn calls the mean is 1 % above the best form tried, one in ten is more than 5 % above it, the worst 1.34 times).  The sequences' own lengths are not known
 // here: a little over half the caches' room.
 //  * own_kernel alone: 4.5, and what it reads (the prefix for every sequence, from L2) at 7 TB/s or a warp's blocks of 16 keys at 0.8 each.
 //    (32 / 8 heads of 128, 4 sequences, 512 keys in front: 6.5 against 9.0 with the prefix apart; 32 sequences, 2000 keys: 41 against 17.)

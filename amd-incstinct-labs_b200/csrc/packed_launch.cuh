@@ -65,8 +65,7 @@ template <int E> __device__ __forceinline__ void load_part(const float* at, floa
 
 // Row r = token * nQH + head from part_o[s][r][D] and part_ml[s][r].  m = max m_s, O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s;
 // parts without a key do not count, a row without any gives zeros.  first, last: device words with the first row to be written and the one
-// behind the last, in tokens, or null.  A warp per row; of many parts, a row's four warps take every fourth (86 parts of 32 rows of 64, the whole
-// call: 18.8 -> 10.4 us; a part's load is L2 latency, and few rows have few warps to hide it).
+// behind the last, in tokens, or null.  A warp per row; or, for few rows and for many parts (launch_merge), four that take every fourth part.
 template <typename T, int D, bool MANY>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int parts, int tokens, int nQH, T* __restrict__ o, long long o_token, long long o_head,
@@ -142,8 +141,10 @@ int launch_after(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A.
 template <typename T, int D>
 int launch_merge(const float* part_o, const float* part_ml, int parts, int tokens, int nQH, void* o, long long o_token, long long o_head, const int* first, const int* last,
                  cudaStream_t st) {
+    // A part's load is L2 latency, which few rows have few warps to hide.  Whole calls of decode behind a prefix, a warp and four per row, us: 32 rows
+    // of 86 parts 18.8 and 10.4; 102 of 12 11.6 and 9.9; 1536 of 9 19.2 and 18.7; but 948 of 3 10.7 and 11.2; 3360 of 8 22.8 and 25.2; 8192 of 5 140 and 145.
     const long long rows = (long long)tokens * nQH, ctas = (rows + kMergeWarps - 1) / kMergeWarps;
-    if (parts <= kFewParts)
+    if (parts <= kFewParts && rows > 220LL * parts)
         return launch_after(merge_kernel<T, D, false>, dim3(unsigned(ctas)), kMergeWarps * 32, st, part_o, part_ml, parts, tokens, nQH, static_cast<T*>(o), o_token, o_head, first, last);
     return launch_after(merge_kernel<T, D, true>, dim3(unsigned(rows)), kMergeWarps * 32, st, part_o, part_ml, parts, tokens, nQH, static_cast<T*>(o), o_token, o_head, first, last);
 }
