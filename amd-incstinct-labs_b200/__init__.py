@@ -654,6 +654,9 @@ def prefill_packed(Q, K, V, q_offsets, k_offsets=None, causal: bool = True, scal
     return out
 
 
+_SHARED_SIZES = {}       # (arguments, device) -> bytes of scratch: a decode loop asks for the same sizes at every step
+
+
 def _shared_args(q, K_prefix, V_prefix, K, V, prefix_len, scale, out):
     if _torch is None:
         _bind()
@@ -703,9 +706,21 @@ def decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len=None, scale: 
     if lengths.shape != q.shape[:1]:
         raise ValueError("lengths has one entry per sequence")
     L = lib()
-    ws = _scratch(workspace, L.b200p_attn_decode_shared_workspace_bytes, a, q, device)
-    _check(_on(device, L.b200p_attn_decode_shared, q.data_ptr(), K_prefix.data_ptr(), V_prefix.data_ptr(), K.data_ptr(), V.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-               a, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(q)), "attn_decode_shared")
+    call = (q.data_ptr(), K_prefix.data_ptr(), V_prefix.data_ptr(), K.data_ptr(), V.data_ptr(), lengths.data_ptr(), out.data_ptr(), a)
+    n = _SHARED_SIZES.get((a, device)) if workspace is None else None
+    if n is None:
+        ws = _scratch(workspace, L.b200p_attn_decode_shared_workspace_bytes, a, q, device)
+        if workspace is None:
+            if len(_SHARED_SIZES) >= 256:
+                _SHARED_SIZES.clear()
+            _SHARED_SIZES[a, device] = 0 if ws is None else ws.nbytes
+    else:
+        ws = q.new_empty(n, dtype=_torch.uint8) if n else None
+    status = _on(device, L.b200p_attn_decode_shared, *call, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes, _stream(q))
+    if status == -7 and n is not None:                            # refused ahead of any launch: a tuning was set since
+        _SHARED_SIZES.clear()
+        return decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len, scale, out)
+    _check(status, "attn_decode_shared")
     return out
 
 

@@ -1,4 +1,4 @@
-"""Checker for the operators of ragged batches, in 64 bits from the formulas, with how far a kernel may be off.
+"""Oracle for the operators of ragged batches, in 64 bits from the formulas, with how far a kernel may be off.
 
 The bounds count roundings.  With A = sum_j p_j |v_j| (the weights are positive and sum to 1) an output is off by at most
   u |o|        its own rounding, u = eps / 2 of the 16-bit type,

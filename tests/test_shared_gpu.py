@@ -49,6 +49,22 @@ def test_every_form(b200p, torch_cuda, batch, heads, kv, D, prefix, own, form, s
     close(got, *ref.shared(*x, n, prefix))
 
 
+def test_a_tuning_between_calls_of_one_size(b200p, torch_cuda):
+    """The scratch's size, which later calls of the same sizes take over from the first, follows the tunings."""
+    torch = torch_cuda
+    x = make(torch, 5, 8, 2, 64, 700, 50, torch.float16, seed=3)
+    n = spread(5, 50)
+    lengths = torch.tensor(n, dtype=torch.int32, device="cuda")
+    want, bound = ref.shared(*x, n, 700)
+    try:
+        for splits in (1, 6, 2, 4, -1, 5):
+            b200p.set_tuning("shared_prefix", 2 if splits > 0 else 1), b200p.set_tuning("shared_splits", splits)
+            for _ in range(2):
+                close(b200p.decode_shared(*x, lengths), want, bound)
+    finally:
+        b200p.set_tuning("shared_prefix", -1), b200p.set_tuning("shared_splits", -1)
+
+
 # long caches of few sequences, long prefixes, both
 @pytest.mark.parametrize("batch,heads,kv,D,prefix,own", [(1, 8, 1, 128, 9000, 5000), (2, 8, 2, 64, 300, 9001), (2, 4, 4, 128, 20000, 10), (64, 8, 2, 128, 4096, 500)])
 def test_long(b200p, torch_cuda, batch, heads, kv, D, prefix, own):
