@@ -271,7 +271,7 @@ own_kernel(const OwnParams p) {
     const int parts = ctas > 1 ? ctas : kOwnWarps;
     const size_t part0 = size_t(b) * nQH + head0, next = size_t(p.batch) * nQH;
     for (int row = warp; row < rows; row += kOwnWarps) {
-        float2 ml = make_float2(-INFINITY, 0.f), pml = ml;
+        float2 ml = make_float2(-INFINITY, 0.f), pml = make_float2(-INFINITY, kNoKey);
         if (lane < p.joined) pml = __ldcg(reinterpret_cast<const float2*>(&p.part_ml[2 * (part0 + row + lane * next)]));
         if (lane < parts)
             ml = ctas > 1 ? make_float2(load_cluster_f32(dme::smem_addr(&s_sum_ml[row][0]), lane), load_cluster_f32(dme::smem_addr(&s_sum_ml[row][1]), lane))
@@ -279,13 +279,13 @@ own_kernel(const OwnParams p) {
         float most = fmaxf(ml.x, pml.x);
         #pragma unroll
         for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        const float f = ml.y == 0.f ? 0.f : weight_of(ml.x, most), g = pml.y <= 0.f ? 0.f : weight_of(pml.x, most);     // no key, or nothing but scores of -inf
-        float sum = f * ml.y + (g == 0.f ? 0.f : g * pml.y);
+        const float f = weight_of(ml.x, most), g = part_weight(pml, most);
+        float sum = f * ml.y + (g == kNoKey ? 0.f : g * pml.y);
         #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         const float inv = p.joined + p.prefix_here + own > 0 ? 1.f / sum : 0.f;
         if (lane < parts) s_w[row][lane] = f * inv;
-        if (lane < p.joined) s_w[row][kMostOwnCluster + lane] = g == 0.f && inv < INFINITY ? 0.f : g * inv;
+        if (lane < p.joined) s_w[row][kMostOwnCluster + lane] = g == kNoKey ? kNoKey : g * inv;
     }
     __syncthreads();
     // four columns per thread
@@ -300,7 +300,7 @@ own_kernel(const OwnParams p) {
             float v[4];
             load_part<4>(at + k * next * D, v);
             #pragma unroll
-            for (int e = 0; e < 4; ++e) if (f != 0.f) x[e] += f * v[e];           // where there was no key nothing was stored
+            for (int e = 0; e < 4; ++e) if (f != kNoKey) x[e] += f * v[e];
         }
         for (int k = 0; k < parts; ++k) {
             const float4 v = ctas > 1 ? load_cluster_f32x4(dme::smem_addr(&s_o[0][row][d]), k) : *reinterpret_cast<const float4*>(&s_o[k][row][d]);

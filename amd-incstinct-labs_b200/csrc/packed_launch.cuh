@@ -63,6 +63,11 @@ template <int E> __device__ __forceinline__ void load_part(const float* at, floa
     else asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "l"(at) : "memory");
 }
 
+// The weight of a part with maximum and sum `ml` beside the maximum of all, or kNoKey for a part without keys, whose O is not stored.  Any other part
+// counts, with a weight of 0 too: where its keys gave no number its maximum may be -inf, or far below the others', and what is no number
+// is none in the row, as it is without splits.
+__device__ __forceinline__ float part_weight(float2 ml, float most) { return ml.y == kNoKey ? kNoKey : weight_of(ml.x, most); }
+
 // Row r = token * nQH + head from part_o[s][r][D] and part_ml[s][r].  m = max m_s, O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s;
 // parts without a key do not count, a row without any gives zeros.  first, last: device words with the first row to be written and the one
 // behind the last, in tokens, or null.  A warp per row; or, for few rows and for many parts (launch_merge), four that take every fourth part.
@@ -92,8 +97,8 @@ merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml
     float sum = 0.f;
     #pragma unroll
     for (int k = 0; k < P; ++k) {
-        const float f = ml[k].y <= 0.f ? 0.f : weight_of(ml[k].x, most);        // no key, or nothing but scores of -inf
-        sum += f == 0.f ? 0.f : f * ml[k].y;
+        const float f = part_weight(ml[k], most);
+        if (f != kNoKey) sum += f * ml[k].y;
         s_f[warp][32 * k + lane] = f;
     }
     #pragma unroll
@@ -106,7 +111,7 @@ merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml
         load_part<E>(part_o + (size_t(s) * rows + row) * D + lane * E, v);
         const float f = s_f[warp][s];
         #pragma unroll
-        for (int e = 0; e < E; ++e) if (f != 0.f) x[e] += f * v[e];             // where there was no key nothing was stored
+        for (int e = 0; e < E; ++e) if (f != kNoKey) x[e] += f * v[e];
     }
     if constexpr (MANY) {
         #pragma unroll

@@ -258,3 +258,38 @@ def test_nothing_to_do(b200p, torch_cuda, splits):
     out = torch.full_like(Q, 7.0)
     assert (b200p.prefill_packed(Q, K, V, torch.zeros(1, dtype=torch.int32, device="cuda"), out=out) == 7.0).all()
     assert (b200p.prefill_packed(Q, K, V, torch.zeros(3, dtype=torch.int32, device="cuda"), out=out) == 7.0).all()
+
+
+# Bad numbers that are seen, all of them in keys of one split: the row has no answer, however the keys are taken.
+@pytest.mark.parametrize("way", ["chosen", 1, 2, 3, 7])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("first,last", [(128, 256), (0, 128), (300, 301)])
+def test_bad_keys_that_fill_a_split(b200p, torch_cuda, first, last, D, causal, way):
+    torch = torch_cuda
+    new, keys = [4, 6, 3], [512, 256, 100]
+    Q, K, V, qo, ko = make(torch, new, keys, 4, 2, D, torch.bfloat16)
+    want, bound = ref.packed(Q, K, V, at(new), at(keys), causal)
+    K[first:last] = math.nan                                      # of the first sequence
+    b200p.set_tuning("packed_splits", -1 if way == "chosen" else way)
+    try:
+        got = b200p.prefill_packed(Q, K, V, qo, ko, causal=causal)
+    finally:
+        b200p.set_tuning("packed_splits", -1)
+    assert got[:4].isnan().all()
+    close(got[4:], want[4:], bound[4:])
+
+
+def test_a_bad_value_whose_weight_is_zero(b200p, torch_cuda, splits):
+    """Zero times what is no number is none: in a split whose keys weigh nothing beside another's as well."""
+    torch = torch_cuda
+    Q, K, V, qo, ko = make(torch, [5], [512], 2, 1, 64, torch.bfloat16)
+    Q[:, :, 0], K[:, :, 0] = 100.0, -100.0
+    K[:100, :, 0] = 100.0                                         # the scores of these are 2500 above the others'
+    V[400, :, 7] = math.nan
+    got = b200p.prefill_packed(Q, K, V, qo, ko)
+    assert got[:, :, 7].isnan().all()
+    V[400, :, 7] = 0.0
+    want, bound = ref.packed(Q, K, V, [0, 5], [0, 512], True)
+    keep = [c for c in range(64) if c != 7]
+    close(got[:, :, keep], want[:, :, keep], bound[:, :, keep])

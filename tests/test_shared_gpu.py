@@ -211,3 +211,47 @@ def test_empty_batch(b200p, torch_cuda):
     torch = torch_cuda
     x = make(torch, 0, 4, 2, 64, 10, 5, torch.bfloat16)
     assert b200p.decode_shared(*x, torch.zeros(0, dtype=torch.int32, device="cuda")).shape == (0, 4, 64)
+
+
+@pytest.fixture(params=[(-1, -1), (1, -1), (2, 1), (2, 4), (2, 12), (3, 1), (3, 4)], ids=lambda p: f"form {p[0]}, {p[1]} splits")
+def form(b200p, request):
+    """The ways to run a call: the prefix per sequence, merged in a launch of its own, merged with the own keys."""
+    b200p.set_tuning("shared_prefix", request.param[0]), b200p.set_tuning("shared_splits", request.param[1])
+    yield request.param
+    b200p.set_tuning("shared_prefix", -1), b200p.set_tuning("shared_splits", -1)
+
+
+# Bad numbers that are seen, all of them in one part: the row has no answer, whichever part it is.
+@pytest.mark.parametrize("batch,heads,kv,D,own", [(5, 8, 2, 128, 40), (5, 6, 1, 64, 700), (60, 16, 1, 128, 33)])
+def test_bad_keys_that_fill_a_part(b200p, torch_cuda, form, batch, heads, kv, D, own):
+    torch = torch_cuda
+    q, Kp, Vp, K, V = make(torch, batch, heads, kv, D, 1500, own, torch.bfloat16)
+    n = spread(batch, own)
+    n[1], n[2], n[3] = 1, own, 0
+    lengths = torch.tensor(n, dtype=torch.int32, device="cuda")
+    want, bound = ref.shared(q, Kp, Vp, K, V, n, 1500)
+    K[1, :, 0], K[2], K[3] = math.nan, math.nan, math.nan         # the only own key; all own keys; keys that nobody sees
+    got = b200p.decode_shared(q, Kp, Vp, K, V, lengths)
+    assert got[1].isnan().all() and got[2].isnan().all()
+    others = [b for b in range(batch) if b not in (1, 2)]
+    close(got[others], want[others], bound[others])
+    for first, last in ((0, 384), (1408, 1500), (700, 701)):
+        bad = Kp.clone()
+        bad[:, first:last] = math.nan
+        assert b200p.decode_shared(q, bad, Vp, K, V, lengths).isnan().all()
+
+
+def test_a_bad_value_whose_weight_is_zero(b200p, torch_cuda, form):
+    """Zero times what is no number is none: in a part whose keys weigh nothing beside another's as well."""
+    torch = torch_cuda
+    q, Kp, Vp, K, V = make(torch, 3, 4, 2, 64, 900, 20, torch.bfloat16)
+    q[:, :, 0], Kp[:, :, 0], K[..., 0] = 100.0, -100.0, -100.0
+    Kp[:, :50, 0] = 100.0                                         # the scores of these are 2500 above the others'
+    Vp[:, 880, 7], V[1, :, 3, 9] = math.nan, math.nan
+    got = b200p.decode_shared(q, Kp, Vp, K, V, torch.tensor([20, 4, 0], dtype=torch.int32, device="cuda"))
+    assert got[:, :, 7].isnan().all() and got[1, :, 9].isnan().all()
+    Vp[:, 880, 7], V[1, :, 3, 9] = 0.0, 0.0
+    want, bound = ref.shared(q, Kp, Vp, K, V, [20, 4, 0], 900)
+    for b in range(3):
+        keep = [c for c in range(64) if c != 7 and (b, c) != (1, 9)]
+        close(got[b][:, keep], want[b][:, keep], bound[b][:, keep])
