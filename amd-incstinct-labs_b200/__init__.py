@@ -962,8 +962,8 @@ class Session:
 
     def set_rules(self, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias=None, allowed=None, banned=None):
         """Rules on generate()'s logits, for all sequences, as adjust_logits has them: penalties for tokens of the prompt and of
-        the answer so far, bias {token: value}, allowed tokens (all others are never picked) and banned ones.  Without arguments the
-        rules are taken back.  The other calls return logits without rules."""
+        the answer so far, bias {token: value}, allowed tokens (all others are never picked) and banned ones, which must leave some token.
+        Without arguments the rules are taken back.  The other calls return logits without rules."""
         import numpy as np
         bias = dict(bias or {})
         V = self.cfg["vocab_size"]

@@ -622,6 +622,12 @@ extern "C" int b200p_session_set_rules(b200p_session* s, const b200p_session_rul
     if (!ids_exist(s, r->bias_ids, size_t(r->bias_n))) return B200P_E_RANGE;
     for (int i = 0; i < r->bias_n; ++i) if (std::isnan(r->bias_values[i])) return B200P_E_RANGE;
     const size_t B = size_t(s->batch), words = (size_t(s->c.vocab_size) + 31) / 32;
+    if (r->mask) {                                              // some token has to be left
+        const unsigned tail = s->c.vocab_size % 32 ? (1u << (s->c.vocab_size % 32)) - 1 : ~0u;
+        bool some = (r->mask[words - 1] & tail) != 0;
+        for (size_t i = 0; i + 1 < words && !some; ++i) some = r->mask[i] != 0;
+        if (!some) return B200P_E_RANGE;
+    }
     auto& d = s->rules;
     if (!d.mask) {
         cudaError_t e;

@@ -110,7 +110,7 @@ int b200p_session_generate(b200p_session* s, const int* input_ids, int T, int ma
  * and the tokens generated in the call as the history.  bias_ids and bias_values: host, bias_n entries (at most
  * 1024); mask: host, (vocab + 31) / 32 words, token t in bit t % 32 of word t / 32, or NULL.  rules = NULL takes them
  * back.  The other calls return logits without rules.  B200P_E_RANGE for a repetition that is not positive, values
- * that are no numbers, ids that do not exist. */
+ * that are no numbers, ids that do not exist, a mask that allows no token. */
 typedef struct b200p_session_rules {
     float repetition;          /* 1: none */
     float presence, frequency; /* 0: none */

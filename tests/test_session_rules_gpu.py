@@ -145,3 +145,21 @@ def test_generate_program(torch_cuda):
     assert {int(t) for t in biased.stdout.split()} == {17}
     assert run("--repetition-penalty", "1.0").stdout == plain.stdout
     assert run("--repetition-penalty", "-1").returncode != 0
+
+
+def test_a_mask_that_leaves_nothing_is_refused(b200p, torch_cuda):
+    torch = torch_cuda
+    cfg = dict(SMALL, vocab_size=SMALL["vocab_size"] - 3)            # bits behind the vocabulary in the mask's last word
+    V = cfg["vocab_size"]
+    assert V % 32
+    s = b200p.Session(cfg, to_device(torch, rr.make_weights(cfg, seed=5, kind="bf16", std=0.05), "bf16"), 64, 1)
+    ids = np.random.default_rng(4).integers(0, V, (1, 20)).astype(np.int32)
+    s.set_rules(bias={9: 100.0})
+    for bad in (dict(allowed=[]), dict(banned=range(V)), dict(allowed=[3, V - 1], banned=[V - 1, 3])):
+        with pytest.raises(b200p.B200PError) as e:
+            s.set_rules(**bad)
+        assert e.value.status == -10
+    assert (s.generate(ids, 4)[0] == 9).all()                        # the old rules
+    s.set_rules(allowed=[V - 1])
+    assert (s.generate(ids, 4)[0] == V - 1).all()
+    s.close()
