@@ -82,10 +82,12 @@ __global__ void embed_gather_kernel(const T* __restrict__ embed, const int* __re
 // (order-preserving value bits, then the complemented index) and merges it into keys[row] with
 // atomicMax; the last block of a row to arrive (ticket counter) writes the id for the next
 // step and the output token, and clears key and counter for the next launch.
-template <typename T>
+// RULES: the logits are adjusted ones.  Tokens whose bit in `mask` (may be null) is 0 are no candidates: one that is allowed may be as low
+// as they are.  What rounds to an infinity counts by its 32 bits, which keep the order.
+template <typename T, bool RULES>
 __global__ void argmax_kernel(const float* __restrict__ logits, int V, int* __restrict__ next_ids,
                               int* __restrict__ tokens, int tokens_stride, int step, const int* __restrict__ step_dev,
-                              unsigned long long* __restrict__ keys, unsigned int* __restrict__ tickets) {
+                              unsigned long long* __restrict__ keys, unsigned int* __restrict__ tickets, const unsigned* __restrict__ mask) {
     griddep_launch_dependents();
     if (step_dev) step = min(*step_dev, tokens_stride - 1);
     __shared__ unsigned long long red[32];
@@ -95,7 +97,9 @@ __global__ void argmax_kernel(const float* __restrict__ logits, int V, int* __re
     const int i0 = blockIdx.y * per, i1 = min(i0 + per, V);
     unsigned long long best = 0;
     for (int i = i0 + threadIdx.x; i < i1; i += blockDim.x) {
-        const float v = to_float(from_float<T>(row[i]));                 // the reference's logits are 16-bit
+        if (RULES && mask && !(mask[i >> 5] >> (i & 31) & 1u)) continue;
+        float v = to_float(from_float<T>(row[i]));                       // the reference's logits are 16-bit
+        if (RULES && isinf(v)) v = row[i];
         unsigned u = __float_as_uint(v);
         u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);                  // order-preserving key
         const unsigned long long key = (unsigned long long)u << 32 | (0xffffffffu - unsigned(i));
@@ -315,8 +319,9 @@ int sample(b200p_session* s, int max_new, int step, const int* step_dev, cudaStr
     }
     return with_type(s->dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        argmax_kernel<T><<<dim3(unsigned(s->batch), unsigned((V + 2047) / 2048)), 256, 0, st>>>(
-            s->logits, V, s->d_next, s->d_tokens, max_new, step, step_dev, s->d_keys, s->d_tickets);
+        const auto kern = s->rules.on ? argmax_kernel<T, true> : argmax_kernel<T, false>;
+        kern<<<dim3(unsigned(s->batch), unsigned((V + 2047) / 2048)), 256, 0, st>>>(
+            s->logits, V, s->d_next, s->d_tokens, max_new, step, step_dev, s->d_keys, s->d_tickets, s->rules.on && s->rules.masked ? s->rules.mask : nullptr);
         return launched();
     });
 }

@@ -106,8 +106,9 @@ int b200p_session_generate(b200p_session* s, const int* input_ids, int T, int ma
                            int* out_tokens, float* timings_ms, b200p_stream_t stream);
 
 /* Rules on the logits of b200p_session_generate, the same for every sequence (b200p_logits_adjust, b200p.h, says
- * what each does): from the next call on the token picked is the largest adjusted logit, with the call's prompt
- * and the tokens generated in the call as the history.  bias_ids and bias_values: host, bias_n entries (at most
+ * what each does): from the next call on the token picked is the largest adjusted logit (rounded to the session's
+ * type where that has room for it) of those that the mask allows, with the call's prompt and the tokens generated in
+ * the call as the history.  bias_ids and bias_values: host, bias_n entries (at most
  * 1024); mask: host, (vocab + 31) / 32 words, token t in bit t % 32 of word t / 32, or NULL.  rules = NULL takes them
  * back.  The other calls return logits without rules.  B200P_E_RANGE for a repetition that is not positive, values
  * that are no numbers, ids that do not exist, a mask that allows no token. */

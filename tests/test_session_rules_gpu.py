@@ -163,3 +163,23 @@ def test_a_mask_that_leaves_nothing_is_refused(b200p, torch_cuda):
     s.set_rules(allowed=[V - 1])
     assert (s.generate(ids, 4)[0] == V - 1).all()
     s.close()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_tokens_that_are_not_allowed_are_never_picked(b200p, torch_cuda, kind):
+    """Adjusted logits outside the session's 16-bit type, in both directions: the largest allowed one is picked."""
+    torch = torch_cuda
+    s = b200p.Session(SMALL, to_device(torch, rr.make_weights(SMALL, seed=5, kind=kind, std=0.05), kind), 96, 2)
+    ids = np.random.default_rng(4).integers(0, SMALL["vocab_size"], (2, 20)).astype(np.int32)
+    far = 1e5 if kind == "f16" else 3.4e38                          # rounds to infinity in the type
+    s.set_rules(allowed=[700, 300, 301], presence=far)               # after the first tokens every allowed one is that far down
+    got = s.generate(ids, 12)[0]
+    assert set(got.ravel()) <= {300, 301, 700}
+    assert all(set(row[:3]) == {300, 301, 700} for row in got)       # each is taken once before one comes again
+    s.set_rules(allowed=[40, 50], bias={40: -2 * 1e5, 50: -1e5})
+    assert (s.generate(ids, 6)[0] == 50).all()
+    s.set_rules(bias={40: 1e5, 50: 3e5, 60: 2e5})
+    assert (s.generate(ids, 6)[0] == 50).all()
+    s.set_rules(allowed=[40], bias={40: -float("inf")})              # the only one allowed, whatever is said about it
+    assert (s.generate(ids, 6)[0] == 40).all()
+    s.close()
