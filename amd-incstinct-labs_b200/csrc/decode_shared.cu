@@ -352,7 +352,7 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
     const int tokens = kBM / group, tiles = (a.batch + tokens - 1) / tokens, steps = (a.prefix_len + kBN - 1) / kBN, fixed = tuning(KNOB_SHARED_SPLITS, 0);
     double best = 0;
     int splits = 0, span = 0;
-    const int first = fixed > 0 ? fixed : kMostSplits;
+    const int first = fixed > 0 && fixed < kMostSplits ? fixed : kMostSplits;
     for (int per = (steps + first - 1) / first, next; per > 0; per = next) {    // key tiles of an item; the next is the smallest with fewer splits
         const int s = (steps + per - 1) / per;
         next = s > 1 && fixed == 0 ? (steps + s - 2) / (s - 1) : 0;

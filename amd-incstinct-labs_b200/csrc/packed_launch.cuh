@@ -146,6 +146,7 @@ int launch_after(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A.
 template <typename T, int D>
 int launch_merge(const float* part_o, const float* part_ml, int parts, int tokens, int nQH, void* o, long long o_token, long long o_head, const int* first, const int* last,
                  cudaStream_t st) {
+    if (parts > kMostParts) return B200P_E_RANGE;
     // A part's load is L2 latency, which few rows have few warps to hide.  Whole calls of decode behind a prefix, a warp and four per row, us: 32 rows
     // of 86 parts 18.8 and 10.4; 102 of 12 11.6 and 9.9; 1536 of 9 19.2 and 18.7; but 948 of 3 10.7 and 11.2; 3360 of 8 22.8 and 25.2; 8192 of 5 140 and 145.
     const long long rows = (long long)tokens * nQH, ctas = (rows + kMergeWarps - 1) / kMergeWarps;

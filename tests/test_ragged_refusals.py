@@ -127,3 +127,20 @@ def test_wrappers_check_shapes_first(b200p):
         with pytest.raises(ValueError):
             b200p._shared_args(*bad, 0.0, bad[0])
     b200p._shared_args(q, Kp, Kp, K, K, 7, 0.0, q)
+
+
+@pytest.mark.parametrize("splits", [1, 152, 153, 400, 1 << 30])
+@pytest.mark.parametrize("prefix", [100, 19456, 32768, 65536, 10 ** 6])
+@pytest.mark.parametrize("form", [2, 3])
+def test_splits_asked_for_are_bounded(b200p, form, prefix, splits):
+    """Scratch for as many parts as a merge takes, and no more, whatever number is asked for: 160, of which the own keys have 8."""
+    try:
+        b200p.set_tuning("shared_prefix", form), b200p.set_tuning("shared_splits", splits)
+        n = b200p.lib().b200p_attn_decode_shared_workspace_bytes(C.byref(shared(b200p, prefix_len=prefix)))
+    finally:
+        b200p.set_tuning("shared_prefix", -1), b200p.set_tuning("shared_splits", -1)
+    row = 3 * 8 * (128 + 2) * 4                         # of a part: batch x heads x (values, maximum and sum)
+    parts = n // row
+    assert 0 <= n - parts * row < 512                   # two arrays of whole 256 bytes
+    tiles = -(-prefix // 128)
+    assert 1 <= parts <= min(splits, tiles, 152) + 8

@@ -255,3 +255,17 @@ def test_a_bad_value_whose_weight_is_zero(b200p, torch_cuda, form):
     for b in range(3):
         keep = [c for c in range(64) if c != 7 and (b, c) != (1, 9)]
         close(got[b][:, keep], want[b][:, keep], bound[b][:, keep])
+
+
+@pytest.mark.parametrize("form,splits", [(2, 1000), (2, 152), (3, 1000), (3, 32), (2, 33)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_splits_than_a_merge_takes(b200p, torch_cuda, form, splits, D):
+    torch = torch_cuda
+    x = make(torch, 3, 6, 2, D, 32768, 700, torch.bfloat16)
+    n = [700, 0, 333]
+    try:
+        b200p.set_tuning("shared_prefix", form), b200p.set_tuning("shared_splits", splits)
+        got = b200p.decode_shared(*x, torch.tensor(n, dtype=torch.int32, device="cuda"))
+    finally:
+        b200p.set_tuning("shared_prefix", -1), b200p.set_tuning("shared_splits", -1)
+    close(got, *ref.shared(*x, n, 32768))
