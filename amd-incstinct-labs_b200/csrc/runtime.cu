@@ -634,23 +634,23 @@ extern "C" int b200p_session_set_rules(b200p_session* s, const b200p_session_rul
         if (!some) return B200P_E_RANGE;
     }
     auto& d = s->rules;
-    if (!d.mask) {
-        cudaError_t e;
-        if ((e = s->alloc(&d.repetition, B * 4)) || (e = s->alloc(&d.presence, B * 4)) || (e = s->alloc(&d.frequency, B * 4)) || (e = s->alloc(&d.mask_rows, B * 4)) ||
-            (e = s->alloc(&d.bias_ids, B * kMostBias * 4)) || (e = s->alloc(&d.bias_values, B * kMostBias * 4)) || (e = cudaMemset(d.mask_rows, 0, B * 4)) ||
-            (e = s->alloc(&d.mask, words * 4))) return int(e);                       // the last: its pointer says that all are there
-    }
-    d.on = false;
-    drop_step_graph(s);
     const std::vector<float> rep(B, r->repetition), pres(B, r->presence), freq(B, r->frequency);
     std::vector<int> ids; std::vector<float> values;
     for (size_t b = 0; b < B; ++b) { ids.insert(ids.end(), r->bias_ids, r->bias_ids + r->bias_n); values.insert(values.end(), r->bias_values, r->bias_values + r->bias_n); }
-    cudaError_t e;
-    if ((e = cudaMemcpy(d.repetition, rep.data(), B * 4, cudaMemcpyHostToDevice)) || (e = cudaMemcpy(d.presence, pres.data(), B * 4, cudaMemcpyHostToDevice)) ||
+    cudaError_t e = cudaSuccess;
+    auto failed = [&] { cudaGetLastError(); return int(e); };    // the next launch does not find it
+    auto room = [&](auto** p, size_t bytes) { return *p || (e = s->alloc(p, bytes)) == cudaSuccess; };       // kept if a later one cannot be had
+    if (!room(&d.repetition, B * 4) || !room(&d.presence, B * 4) || !room(&d.frequency, B * 4) || !room(&d.mask_rows, B * 4) || !room(&d.bias_ids, B * kMostBias * 4) ||
+        !room(&d.bias_values, B * kMostBias * 4) || !room(&d.mask, words * 4)) return failed();
+    d.on = false;
+    drop_step_graph(s);
+    if ((e = cudaMemset(d.mask_rows, 0, B * 4)) || (e = cudaMemcpy(d.repetition, rep.data(), B * 4, cudaMemcpyHostToDevice)) || (e = cudaMemcpy(d.presence, pres.data(), B * 4, cudaMemcpyHostToDevice)) ||
         (e = cudaMemcpy(d.frequency, freq.data(), B * 4, cudaMemcpyHostToDevice)) ||
         (!ids.empty() && ((e = cudaMemcpy(d.bias_ids, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice)) ||
                           (e = cudaMemcpy(d.bias_values, values.data(), values.size() * 4, cudaMemcpyHostToDevice)))) ||
-        (r->mask && (e = cudaMemcpy(d.mask, r->mask, words * 4, cudaMemcpyHostToDevice)))) return int(e);
+        (r->mask && (e = cudaMemcpy(d.mask, r->mask, words * 4, cudaMemcpyHostToDevice)))) return failed();
+    // a copy from pageable memory may still be under way, and the next call's stream need not be ordered behind the default one
+    if ((e = cudaStreamSynchronize(cudaStreamLegacy))) return failed();
     d.bias_n = r->bias_n; d.masked = r->mask != nullptr;
     d.on = true;
     return B200P_OK;

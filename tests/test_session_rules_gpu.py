@@ -183,3 +183,20 @@ def test_tokens_that_are_not_allowed_are_never_picked(b200p, torch_cuda, kind):
     s.set_rules(allowed=[40], bias={40: -float("inf")})              # the only one allowed, whatever is said about it
     assert (s.generate(ids, 6)[0] == 40).all()
     s.close()
+
+
+def test_rules_set_just_ahead_of_a_call_on_another_stream(b200p, torch_cuda):
+    """set_rules is complete when it returns: no stream's generate() sees half of it."""
+    torch = torch_cuda
+    s = b200p.Session(SMALL, to_device(torch, rr.make_weights(SMALL, seed=5, kind="bf16", std=0.05), "bf16"), 32, 2)
+    ids = np.full((2, 1), 3, np.int32)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for i in range(60):
+        t = (i * 37 + 5) % SMALL["vocab_size"]
+        with torch.cuda.stream(streams[i % 3]):
+            if i % 2:
+                s.set_rules(bias={(t + 1) % SMALL["vocab_size"]: 1000.0, t: 2000.0})
+            else:
+                s.set_rules(allowed=[t], presence=0.5)
+            assert (s.generate(ids, 2)[0] == t).all()
+    s.close()
