@@ -20,6 +20,10 @@ namespace b200p {
 // The next item is looked for when the K tile of this many steps before the item's end is asked for.  (1, 2, 3, 4: no difference.)
 constexpr int kAskAhead = 2;
 
+// What takes a time that grows with the sizes and holds up the CTA's other warps says every so often that it is at work (dme::say_alive), so
+// that their bounded waits (2 s) go on: the walk over very many sequences, an item of very many key tiles, rows done again on long caches.
+constexpr int kAliveChunks = 1024, kAliveTiles = 4096, kAliveKeys = 4096;
+
 constexpr float kNoKey = -1.f;             // in place of a part's sum, whose O is not stored then
 
 struct PackedParams : PrefillParams {      // seqQ, seqK: rows of Q and of K and V; batch: sequences; span, scale_log2, causal, nKVH, group
@@ -81,13 +85,14 @@ __device__ __forceinline__ PackedItem packed_split(const PackedParams& p, int id
 // Finds this CTA's items and calls publish(i, item) for them in order, the last time with kvh = -1, until it returns false.  One warp.
 // answer, bar: shared memory for requests of further CTAs' items.
 template <typename Publish>
-__device__ __forceinline__ bool packed_walk(const PackedParams& p, void* answer, uint64_t* bar, Publish&& publish) {
+__device__ __forceinline__ bool packed_walk(const PackedParams& p, void* answer, uint64_t* bar, uint64_t* alive, Publish&& publish) {
     constexpr unsigned kAll = 0xffffffffu;
     const int lane = threadIdx.x % 32;
     const int block = p.span * p.tokens, chunks = (p.batch + 31) / 32, per = p.nKVH * p.splits;
     int q = 0, k = 0, n = 0, m = 0;                             // this lane's sequence: first rows, lengths
     auto load = [&](int c) {
         const int b = c * 32 + lane;
+        if (c % kAliveChunks == kAliveChunks - 1 && lane == 0) dme::say_alive(alive);
         q = k = n = m = 0;
         if (b >= p.batch) return;
         q = min(max(p.q_offsets[b], 0), p.seqQ); n = min(max(p.q_offsets[b + 1], q), p.seqQ) - q;
@@ -178,13 +183,17 @@ __device__ __forceinline__ bool packed_walk(const PackedParams& p, void* answer,
 // One query row once more, by the whole warp, from the n keys that it sees, and out: PARTIAL as fp32, not divided, with its
 // maximum and sum, else as 16 bits.
 template <typename T, int D, bool PARTIAL>
-__device__ __forceinline__ void packed_row_again(const T* q, const T* K, const T* V, long long k_token, long long v_token, int n, float scale_log2, void* out, float* ml) {
+__device__ __forceinline__ void packed_row_again(const T* q, const T* K, const T* V, long long k_token, long long v_token, int n, float scale_log2, void* out, float* ml,
+                                                 uint64_t* alive) {
     constexpr int E = D / 32;
     const int lane = threadIdx.x % 32;
     float x[E];
     load_part<T, E>(q + lane * E, x);
     RowState<D> st;
-    attend_keys<T, D>(st, x, K, V, k_token, v_token, n, scale_log2);
+    for (int j = 0; j < n; j += kAliveKeys) {
+        attend_keys<T, D>(st, x, K + j * k_token, V + j * v_token, k_token, v_token, min(n - j, kAliveKeys), scale_log2);
+        if (lane == 0) dme::say_alive(alive);
+    }
     if constexpr (PARTIAL) {
         for (int i = 0; i < E; ++i) static_cast<float*>(out)[lane * E + i] = st.o[i];
         if (lane == 0) { ml[0] = st.m; ml[1] = st.l; }
@@ -207,7 +216,8 @@ __device__ __forceinline__ void packed_no_keys(const PackedParams& p, const Pack
 
 // A tile's rows out, a row per thread: v is the thread's row of O, m and l its maximum and sum.
 template <typename T, typename Sh>
-__device__ __forceinline__ void packed_epilogue(const PackedParams& p, const PackedItem& w, uint32_t (&v)[Sh::DV], float m, float l, int nt, int q0, int row_token, bool live, int r) {
+__device__ __forceinline__ void packed_epilogue(const PackedParams& p, const PackedItem& w, uint32_t (&v)[Sh::DV], float m, float l, int nt, int q0, int row_token, bool live, int r,
+                                                uint64_t* alive) {
     constexpr int D = Sh::DV;
     constexpr bool PARTIAL = Sh::PARTIAL;
     const int token = q0 + row_token, g = r - row_token * p.group;
@@ -254,7 +264,7 @@ __device__ __forceinline__ void packed_epilogue(const PackedParams& p, const Pac
         const size_t row = (size_t(w.split) * p.seqQ + w.q_row + tok) * (p.nKVH * p.group) + head;
         void* out = PARTIAL ? static_cast<void*>(p.part_o + row * D) : static_cast<void*>(static_cast<T*>(p.O) + (w.q_row + tok) * p.o_token + head * p.o_head);
         packed_row_again<T, D, PARTIAL>(static_cast<const T*>(p.Q) + (w.q_row + tok) * p.q_token + head * p.q_head, static_cast<const T*>(p.K) + key * p.k_token + w.kvh * p.k_head,
-                                        static_cast<const T*>(p.V) + key * p.v_token + w.kvh * p.v_head, p.k_token, p.v_token, n, p.scale_log2, out, PARTIAL ? p.part_ml + 2 * row : nullptr);
+                                        static_cast<const T*>(p.V) + key * p.v_token + w.kvh * p.v_head, p.k_token, p.v_token, n, p.scale_log2, out, PARTIAL ? p.part_ml + 2 * row : nullptr, alive);
     }
 }
 

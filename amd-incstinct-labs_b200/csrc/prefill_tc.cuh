@@ -193,6 +193,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
     using Item = std::conditional_t<PACKED, PackedItem, PrefillItem>;
     __shared__ std::conditional_t<PACKED, PackedItem, int> s_packed[2];
     __shared__ __align__(16) uint4 s_answer[1];
+    __shared__ uint64_t s_alive;                               // PACKED: for work without a bound in time, of which the others' waits do not tire
 
     constexpr int kMmaWarp = 8 * RS, kTmaWarp = 8 * RS + 1, kWalkWarp = 8 * RS + 2;
     constexpr int kItemReaders = 2 * kBM + 1 + PACKED;         // every softmax thread + the MMA thread; PACKED: + the TMA thread
@@ -209,7 +210,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
             dme::mbar_init(&o_done[t], 1); dme::mbar_init(&o_free[t], kBM);
             dme::mbar_init(&item_full[t], 1); dme::mbar_init(&item_empty[t], kItemReaders);
         }
-        if constexpr (PACKED) { dme::mbar_init(answer_bar, 1); dme::mbar_init(ask_next, 1); }
+        if constexpr (PACKED) { dme::mbar_init(answer_bar, 1); dme::mbar_init(ask_next, 1); s_alive = 0; }
         dme::mbar_init_fence();
     }
     if (warp == kMmaWarp) { tc::tmem_alloc(&s_tmem_base, 512); tc::tmem_relinquish(); }
@@ -227,6 +228,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
     // PACKED: a warp of its own (kWalkWarp) finds the items from the sequences' lengths, which are known on the device only, and
     // publishes them whole.
     int* const abort_word = [&] { if constexpr (PACKED) return &s_failed; else return p.status; }();     // PACKED: no CTA waits for another
+    uint64_t* const alive = [&]() -> uint64_t* { if constexpr (PACKED) return &s_alive; else return nullptr; }();
     auto read_item = [&](int it, Item& w) -> int {             // behind item_full: the CTA's it-th item; its id, or negative: there are no more
         if constexpr (PACKED && !WALK) {                       // known without looking: every role finds them itself
             const int id = int(blockIdx.x) + it * int(gridDim.x);
@@ -240,7 +242,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         }
     };
     auto next_item = [&](int it, Item& w) -> int {             // consumer side
-        if (!(PACKED && !WALK) && !dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word)) return -2;
+        if (!(PACKED && !WALK) && !dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word, alive)) return -2;
         const int id = read_item(it, w);
         if (!(PACKED && !WALK)) dme::mbar_arrive(&item_empty[it & 1]);
         return id;
@@ -267,7 +269,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                     const int id = next_item(it, w);
                     if (id < 0) { ok = id != -2; break; }
                     if (w.nmax == 0) { dme::mbar_arrive(ask_next); continue; }      // rows without keys: only zeros to write
-                    if (worked >= 1 && !dme::wait(q_empty, uint32_t((worked - 1) & 1), abort_word)) { ok = false; break; }
+                    if (worked >= 1 && !dme::wait(q_empty, uint32_t((worked - 1) & 1), abort_word, alive)) { ok = false; break; }
                     ++worked;
                     dme::mbar_arrive_expect_tx(q_full, uint32_t((w.n[0] > 0) + (w.n[1] > 0)) * Sh::QK_SUB * uint32_t(p.tokens * p.group) * 128u);
                 } else {
@@ -291,7 +293,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                         else                  dme::copy_tile_4d(dst, &mapQ, sb * 64, w.q0[t], w.head, w.b, q_full);
                     }
                 for (int j = 0; j < w.nmax; ++j) {
-                    if (kloads >= KST && !dme::wait(&k_empty[kr.stage], kr.phase ^ 1u, abort_word)) { ok = false; break; }
+                    if (kloads >= KST && !dme::wait(&k_empty[kr.stage], kr.phase ^ 1u, abort_word, alive)) { ok = false; break; }
                     dme::mbar_arrive_expect_tx(&k_full[kr.stage], Sh::QK_BYTES);
                     for (int sb = 0; sb < Sh::QK_SUB; ++sb) {
                         unsigned char* dst = smem + Sh::OFF_K + kr.stage * Sh::QK_BYTES + sb * Sh::SUB_BYTES;
@@ -300,8 +302,11 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                         else                  dme::copy_tile_4d(dst, &mapK, sb * 64, (w.first + j) * kBN, w.kvh, w.b, &k_full[kr.stage]);
                     }
                     kr.advance(); ++kloads;
-                    if constexpr (PACKED) if (j == max(w.nmax - kAskAhead, 0)) dme::mbar_arrive(ask_next);
-                    if (vloads >= VST && !dme::wait(&v_empty[vr.stage], vr.phase ^ 1u, abort_word)) { ok = false; break; }
+                    if constexpr (PACKED) {
+                        if (j % kAliveTiles == kAliveTiles - 1) dme::say_alive(alive);       // the walk waits until the item's end is near
+                        if (j == max(w.nmax - kAskAhead, 0)) dme::mbar_arrive(ask_next);
+                    }
+                    if (vloads >= VST && !dme::wait(&v_empty[vr.stage], vr.phase ^ 1u, abort_word, alive)) { ok = false; break; }
                     dme::mbar_arrive_expect_tx(&v_full[vr.stage], Sh::V_BYTES);
                     for (int sb = 0; sb < Sh::V_SUB; ++sb) {
                         unsigned char* dst = smem + Sh::OFF_V + vr.stage * Sh::V_BYTES + sb * Sh::SUB_BYTES;
@@ -326,7 +331,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         const uint64_t k_base = tc::smem_desc_sw128(sm_k, 16, 1024);
         const uint64_t v_base = tc::smem_desc_sw128(sm_v, Sh::SUB_BYTES, 1024);
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, dme::wait(bar, parity, abort_word)) != 0; };
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, dme::wait(bar, parity, abort_word, alive)) != 0; };
         auto issue_qk = [&](int t, int kstage) {
             const uint64_t qd = q_base + uint64_t((t * Sh::QK_BYTES) >> 4);
             const uint64_t kd = k_base + uint64_t((kstage * Sh::QK_BYTES) >> 4);
@@ -441,14 +446,14 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
       } else if (WALK && warp == kWalkWarp) {
         if constexpr (WALK) {
             bool ok = true;
-            const bool fine = packed_walk(p, s_answer, answer_bar, [&](int it, const PackedItem& w) -> bool {
-                if (it >= 2) ok = dme::wait(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1), abort_word);
+            const bool fine = packed_walk(p, s_answer, answer_bar, alive, [&](int it, const PackedItem& w) -> bool {
+                if (it >= 2) ok = dme::wait(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1), abort_word, alive);
                 ok = __all_sync(0xffffffffu, ok) != 0;
                 if (ok && lane == 0) { s_packed[it & 1] = w; dme::mbar_arrive(&item_full[it & 1]); }
                 __syncwarp();
                 // a next item is asked for with this one's last steps ahead (kAskAhead): what a busy CTA holds is work that idle ones
                 // miss (6 portions of prompts, 184 items: 157 us when asked for at an item's begin)
-                if (ok && w.kvh >= 0) ok = __all_sync(0xffffffffu, dme::wait(ask_next, uint32_t(it & 1), abort_word)) != 0;
+                if (ok && w.kvh >= 0) ok = __all_sync(0xffffffffu, dme::wait(ask_next, uint32_t(it & 1), abort_word, alive)) != 0;
                 return ok;
             });
             if (!(ok && fine) && lane == 0) atomicExch(&s_failed, 1);
@@ -504,7 +509,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
           if (MASKED) { m_used = p.plus_one ? 0.f : -1e30f; l = p.plus_one ? 1.f : 0.f; }      // finite: a row may see nothing of its first tiles
           if constexpr (PORTION) if (p.sink) { m_used = p.sink[o_head] * 1.4426950408889634f; l = 1.f; }    // one more term of the denominator
           for (int j = 0; j < nt; ++j) {
-            if (!dme::wait(&s_full[t], uint32_t((cs + j) & 1), abort_word)) { ok = false; break; }
+            if (!dme::wait(&s_full[t], uint32_t((cs + j) & 1), abort_word, alive)) { ok = false; break; }
             tc::fence_after_sync();
             if (PACKED && !warp_live) {                          // O's rows of this warp are never read: any P does
                 dme::mbar_arrive(&p_half[2 * t]); dme::mbar_arrive(&p_half[2 * t + 1]);
@@ -582,7 +587,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
           }
           // ---- epilogue: O / l -> 16-bit, through a swizzled staging tile and TMA stores (64 columns at a time).  O is taken
           // into registers first and the tile's tensor memory released, so the next item's P.V does not wait for the stores.
-          if (ok && nt > 0) ok = dme::wait(&o_done[t], uint32_t(co & 1), abort_word);
+          if (ok && nt > 0) ok = dme::wait(&o_done[t], uint32_t(co & 1), abort_word, alive);
           ok = all_of_tile(ok);
           if (!ok) break;
           if constexpr (PACKED) {
@@ -594,7 +599,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                 tc::wait_ld();
                 tc::fence_before_sync();
                 dme::mbar_arrive(&o_free[t]);
-                packed_epilogue<T, Sh>(p, w, v, m_used, l, nt, q0t, row_token, live, r);
+                packed_epilogue<T, Sh>(p, w, v, m_used, l, nt, q0t, row_token, live, r, alive);
             } else if (live) packed_no_keys<T, Sh>(p, w, row, r - row_token * p.group);
           } else if (nt > 0) {
             tc::fence_after_sync();

@@ -293,3 +293,35 @@ def test_a_bad_value_whose_weight_is_zero(b200p, torch_cuda, splits):
     want, bound = ref.packed(Q, K, V, [0, 5], [0, 512], True)
     keep = [c for c in range(64) if c != 7]
     close(got[:, :, keep], want[:, :, keep], bound[:, :, keep])
+
+
+def test_rows_that_take_longer_than_a_wait(b200p, torch_cuda):
+    """Rows done again over a very long cache (32 of them by one warp, 4 to 10 us a key) keep the CTA's other warps waiting for more than
+    their limit of 2 s; the item that the CTA has taken meanwhile is not lost."""
+    torch = torch_cuda
+    new, keys = [32] + [10] * 400, [420000] + [10] * 400
+    Q, K, V, qo, ko = make(torch, new, keys, 1, 1, 64, torch.bfloat16)
+    V[0] = math.nan
+    b200p.set_tuning("packed_splits", 1)
+    try:
+        got = b200p.prefill_packed(Q, K, V, qo, ko)
+    finally:
+        b200p.set_tuning("packed_splits", -1)
+    assert b200p.device_status() == 0
+    assert got[:32].isnan().all()
+    close(got[32:], *ref.packed(Q[32:], K[420000:], V[420000:], at(new[1:]), at(keys[1:]), True))
+
+
+def test_tens_of_thousands_of_sequences(b200p, torch_cuda):
+    torch = torch_cuda
+    batch = 70001
+    new = [(i * 37) % 9 for i in range(batch)]
+    new[40000] = 1500                                             # levels of work that only one sequence has
+    offsets = [0] + torch.tensor(new).cumsum(0).tolist()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    Q, K, V = (torch.randn(offsets[-1], h, 64, device="cuda", generator=g).bfloat16() for h in (2, 1, 1))
+    got = b200p.prefill_packed(Q, K, V, torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+    assert b200p.device_status() == 0 and got.isfinite().all()
+    for b in list(range(0, batch, 401)) + [40000, 32767, 32768, 32769, batch - 1]:
+        rows = slice(offsets[b], offsets[b + 1])
+        close(got[rows], *ref.packed(Q[rows], K[rows], V[rows], [0, new[b]], [0, new[b]], True))
