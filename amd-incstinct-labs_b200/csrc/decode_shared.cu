@@ -447,6 +447,7 @@ int checked(const b200p_shared_args* args, b200p_shared_args* out) {
     if (a.D != 64 && a.D != 128) return B200P_E_DIM;
     if (a.nQHeads <= 0 || a.nKVHeads <= 0 || a.nQHeads % a.nKVHeads != 0) return B200P_E_DIM;
     if (a.batch < 0 || a.prefix_len < 0 || a.max_own < 0 || !(a.scale >= 0.f) || std::isinf(a.scale)) return B200P_E_LENGTH;
+    if (a.prefix_len > kMostRows || a.max_own > kMostRows) return B200P_E_RANGE;
     if (a.nQHeads / a.nKVHeads > 128 || a.nQHeads > 65535 || a.batch > 65535 || (long long)a.batch * a.nQHeads > (1 << 28)) return B200P_E_RANGE;
     const long long D = a.D;
     if (a.prefix_head == 0) a.prefix_head = a.prefix_len * D;

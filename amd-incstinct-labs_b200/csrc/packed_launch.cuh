@@ -5,6 +5,9 @@
 
 namespace b200p {
 
+// Rows of a tensor at most: counts of rows are rounded up to tiles, and of tiles to levels of work (packed_walk), in 32 bits.
+constexpr int kMostRows = 0x7fffffff - 0xffff;
+
 // Query tiles that all the sequences have at most, over all key heads: each may end inside one.
 inline long long packed_tiles(long long rows, int batch, int tokens, int kv_heads) { return (rows / tokens + batch) * kv_heads; }
 

@@ -76,6 +76,7 @@ int checked(const b200p_packed_args* args, b200p_packed_args* out) {
     if (a.D != 64 && a.D != 128) return B200P_E_DIM;
     if (a.nQHeads <= 0 || a.nKVHeads <= 0 || a.nQHeads % a.nKVHeads != 0) return B200P_E_DIM;
     if (a.batch < 0 || a.total_q < 0 || a.total_k < 0 || !(a.scale >= 0.f) || std::isinf(a.scale)) return B200P_E_LENGTH;
+    if (a.total_q > kMostRows || a.total_k > kMostRows) return B200P_E_RANGE;
     if (a.nQHeads / a.nKVHeads > 128 || a.nQHeads > 65535 || a.batch > (1 << 24) || (long long)a.total_q * a.nQHeads > 0x7fffffffLL) return B200P_E_RANGE;
     const long long D = a.D;
     auto fill = [&](long long& token, long long& head, long long heads) { if (token == 0 && head == 0) { token = heads * D; head = D; } };

@@ -381,7 +381,7 @@ typedef struct b200p_packed_args {
     int nKVHeads;
     int batch;                 /* sequences, at most 2^24; empty ones (no queries, no keys)
                                   are fine                                                */
-    int total_q, total_k;      /* rows of Q and O, rows of K and V                        */
+    int total_q, total_k;      /* rows of Q and O, rows of K and V, at most 2^31 - 2^16   */
     int causal;
     int dtype;                 /* B200P_F16 or B200P_BF16                                 */
     float scale;               /* of the scores; 0 = 1/sqrt(D)                            */
@@ -411,8 +411,8 @@ typedef struct b200p_shared_args {
     int nQHeads;
     int nKVHeads;              /* nQHeads % nKVHeads == 0, at most 128 per key head       */
     int batch;                 /* sequences, at most 65535                                */
-    int prefix_len;            /* keys of the prefix, may be 0                            */
-    int max_own;               /* bound of lengths[], may be 0                            */
+    int prefix_len;            /* keys of the prefix, may be 0; at most 2^31 - 2^16       */
+    int max_own;               /* bound of lengths[], may be 0; at most 2^31 - 2^16       */
     int dtype;                 /* B200P_F16 or B200P_BF16                                 */
     float scale;               /* of the scores; 0 = 1/sqrt(D)                            */
     long long prefix_head;     /* elements between KV heads of K_prefix and V_prefix;

@@ -144,3 +144,15 @@ def test_splits_asked_for_are_bounded(b200p, form, prefix, splits):
     assert 0 <= n - parts * row < 512                   # two arrays of whole 256 bytes
     tiles = -(-prefix // 128)
     assert 1 <= parts <= min(splits, tiles, 152) + 8
+
+
+@pytest.mark.parametrize("far", [(1 << 31) - 1, (1 << 31) - 128, (1 << 31) - (1 << 16) + 1])
+def test_lengths_next_to_32_bits(b200p, far):
+    """Rows are counted in tiles, and tiles in levels of work, in 32 bits."""
+    for name in ("total_q", "total_k"):
+        a = packed(b200p, nQHeads=1, nKVHeads=1, q_token=8, k_token=8, v_token=8, o_token=8, q_head=64, k_head=64, v_head=64, o_head=64, **{name: far})
+        assert call_packed(b200p, a) == E["range"], name
+        assert b200p.lib().b200p_attn_prefill_packed_workspace_bytes(C.byref(a)) == 0
+    for name in ("prefix_len", "max_own"):
+        assert call_shared(b200p, shared(b200p, **{name: far})) == E["range"], name
+        assert b200p.lib().b200p_attn_decode_shared_workspace_bytes(C.byref(shared(b200p, **{name: far}))) == 0
