@@ -227,8 +227,9 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
     // first Q.K^T are under way while the softmax warps still normalise and store the previous item's O.
     // PACKED: a warp of its own (kWalkWarp) finds the items from the sequences' lengths, which are known on the device only, and
     // publishes them whole.
-    int* const abort_word = [&] { if constexpr (PACKED) return &s_failed; else return p.status; }();     // PACKED: no CTA waits for another
     uint64_t* const alive = [&]() -> uint64_t* { if constexpr (PACKED) return &s_alive; else return nullptr; }();
+    // PACKED: no CTA waits for another
+    auto bounded = [&](uint64_t* bar, uint32_t parity) { if constexpr (PACKED) return dme::wait_alive(bar, parity, alive); else return dme::wait(bar, parity, p.status); };
     auto read_item = [&](int it, Item& w) -> int {             // behind item_full: the CTA's it-th item; its id, or negative: there are no more
         if constexpr (PACKED && !WALK) {                       // known without looking: every role finds them itself
             const int id = int(blockIdx.x) + it * int(gridDim.x);
@@ -242,7 +243,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         }
     };
     auto next_item = [&](int it, Item& w) -> int {             // consumer side
-        if (!(PACKED && !WALK) && !dme::wait(&item_full[it & 1], uint32_t((it >> 1) & 1), abort_word, alive)) return -2;
+        if (!(PACKED && !WALK) && !bounded(&item_full[it & 1], uint32_t((it >> 1) & 1))) return -2;
         const int id = read_item(it, w);
         if (!(PACKED && !WALK)) dme::mbar_arrive(&item_empty[it & 1]);
         return id;
@@ -269,7 +270,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                     const int id = next_item(it, w);
                     if (id < 0) { ok = id != -2; break; }
                     if (w.nmax == 0) { dme::mbar_arrive(ask_next); continue; }      // rows without keys: only zeros to write
-                    if (worked >= 1 && !dme::wait(q_empty, uint32_t((worked - 1) & 1), abort_word, alive)) { ok = false; break; }
+                    if (worked >= 1 && !bounded(q_empty, uint32_t((worked - 1) & 1))) { ok = false; break; }
                     ++worked;
                     dme::mbar_arrive_expect_tx(q_full, uint32_t((w.n[0] > 0) + (w.n[1] > 0)) * Sh::QK_SUB * uint32_t(p.tokens * p.group) * 128u);
                 } else {
@@ -293,7 +294,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                         else                  dme::copy_tile_4d(dst, &mapQ, sb * 64, w.q0[t], w.head, w.b, q_full);
                     }
                 for (int j = 0; j < w.nmax; ++j) {
-                    if (kloads >= KST && !dme::wait(&k_empty[kr.stage], kr.phase ^ 1u, abort_word, alive)) { ok = false; break; }
+                    if (kloads >= KST && !bounded(&k_empty[kr.stage], kr.phase ^ 1u)) { ok = false; break; }
                     dme::mbar_arrive_expect_tx(&k_full[kr.stage], Sh::QK_BYTES);
                     for (int sb = 0; sb < Sh::QK_SUB; ++sb) {
                         unsigned char* dst = smem + Sh::OFF_K + kr.stage * Sh::QK_BYTES + sb * Sh::SUB_BYTES;
@@ -306,7 +307,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
                         if (j % kAliveTiles == kAliveTiles - 1) dme::say_alive(alive);       // the walk waits until the item's end is near
                         if (j == max(w.nmax - kAskAhead, 0)) dme::mbar_arrive(ask_next);
                     }
-                    if (vloads >= VST && !dme::wait(&v_empty[vr.stage], vr.phase ^ 1u, abort_word, alive)) { ok = false; break; }
+                    if (vloads >= VST && !bounded(&v_empty[vr.stage], vr.phase ^ 1u)) { ok = false; break; }
                     dme::mbar_arrive_expect_tx(&v_full[vr.stage], Sh::V_BYTES);
                     for (int sb = 0; sb < Sh::V_SUB; ++sb) {
                         unsigned char* dst = smem + Sh::OFF_V + vr.stage * Sh::V_BYTES + sb * Sh::SUB_BYTES;
@@ -331,7 +332,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         const uint64_t k_base = tc::smem_desc_sw128(sm_k, 16, 1024);
         const uint64_t v_base = tc::smem_desc_sw128(sm_v, Sh::SUB_BYTES, 1024);
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, dme::wait(bar, parity, abort_word, alive)) != 0; };
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bounded(bar, parity)) != 0; };
         auto issue_qk = [&](int t, int kstage) {
             const uint64_t qd = q_base + uint64_t((t * Sh::QK_BYTES) >> 4);
             const uint64_t kd = k_base + uint64_t((kstage * Sh::QK_BYTES) >> 4);
@@ -447,13 +448,13 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
         if constexpr (WALK) {
             bool ok = true;
             const bool fine = packed_walk(p, s_answer, answer_bar, alive, [&](int it, const PackedItem& w) -> bool {
-                if (it >= 2) ok = dme::wait(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1), abort_word, alive);
+                if (it >= 2) ok = bounded(&item_empty[it & 1], uint32_t(((it >> 1) - 1) & 1));
                 ok = __all_sync(0xffffffffu, ok) != 0;
                 if (ok && lane == 0) { s_packed[it & 1] = w; dme::mbar_arrive(&item_full[it & 1]); }
                 __syncwarp();
                 // a next item is asked for with this one's last steps ahead (kAskAhead): what a busy CTA holds is work that idle ones
                 // miss (6 portions of prompts, 184 items: 157 us when asked for at an item's begin)
-                if (ok && w.kvh >= 0) ok = __all_sync(0xffffffffu, dme::wait(ask_next, uint32_t(it & 1), abort_word, alive)) != 0;
+                if (ok && w.kvh >= 0) ok = __all_sync(0xffffffffu, bounded(ask_next, uint32_t(it & 1))) != 0;
                 return ok;
             });
             if (!(ok && fine) && lane == 0) atomicExch(&s_failed, 1);
@@ -509,7 +510,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
           if (MASKED) { m_used = p.plus_one ? 0.f : -1e30f; l = p.plus_one ? 1.f : 0.f; }      // finite: a row may see nothing of its first tiles
           if constexpr (PORTION) if (p.sink) { m_used = p.sink[o_head] * 1.4426950408889634f; l = 1.f; }    // one more term of the denominator
           for (int j = 0; j < nt; ++j) {
-            if (!dme::wait(&s_full[t], uint32_t((cs + j) & 1), abort_word, alive)) { ok = false; break; }
+            if (!bounded(&s_full[t], uint32_t((cs + j) & 1))) { ok = false; break; }
             tc::fence_after_sync();
             if (PACKED && !warp_live) {                          // O's rows of this warp are never read: any P does
                 dme::mbar_arrive(&p_half[2 * t]); dme::mbar_arrive(&p_half[2 * t + 1]);
@@ -587,7 +588,7 @@ prefill_tc_kernel(const typename Sh::Params p, const __grid_constant__ CUtensorM
           }
           // ---- epilogue: O / l -> 16-bit, through a swizzled staging tile and TMA stores (64 columns at a time).  O is taken
           // into registers first and the tile's tensor memory released, so the next item's P.V does not wait for the stores.
-          if (ok && nt > 0) ok = dme::wait(&o_done[t], uint32_t(co & 1), abort_word, alive);
+          if (ok && nt > 0) ok = bounded(&o_done[t], uint32_t(co & 1));
           ok = all_of_tile(ok);
           if (!ok) break;
           if constexpr (PACKED) {

@@ -84,10 +84,8 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 // `abort_flag` (optional, global memory): a word that is non-zero once ANY wait of the launch has
 // given up; every other wait then gives up at its next check instead of running out its own limit, so
 // a launch whose pipeline is broken ends within about one limit, not one limit per CTA.
-// `alive` (optional): when a thread that others wait for last said that it is at work (say_alive); the limit counts from then.
-__device__ __forceinline__ void say_alive(uint64_t* alive) { *reinterpret_cast<volatile uint64_t*>(alive) = global_timer_ns(); }
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag = nullptr, const uint64_t* alive = nullptr) {
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag = nullptr) {
     auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
     if (done()) return true;
     const uint64_t t0 = global_timer_ns();
@@ -96,9 +94,28 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_
         for (int i = 0; i < 256; ++i)
             if (done()) return true;
         if (abort_flag && *reinterpret_cast<volatile int*>(abort_flag) != 0) return false;
-        const uint64_t now = global_timer_ns();
-        if (now - t0 > kWaitLimitNs && !(alive && int64_t(now - *reinterpret_cast<const volatile uint64_t*>(alive)) <= int64_t(kWaitLimitNs))) {
+        if (global_timer_ns() - t0 > kWaitLimitNs) {
             if (abort_flag) atomicExch(abort_flag, 1);
+            return false;
+        }
+    }
+}
+// The same among threads that may have to wait for one that is at work for longer than the limit.  `alive` (shared memory, 0 at first): the time
+// at which such a thread last said so; the limit counts from there.  It is the abort word as well: a wait that gives up leaves a time to come
+// there, of which no other is within the limit.
+__device__ __forceinline__ void say_alive(uint64_t* alive) {
+    *reinterpret_cast<volatile uint64_t*>(alive) = global_timer_ns() - 1000000;      // behind every clock that may be read later
+}
+__device__ __forceinline__ bool wait_alive(uint64_t* bar, uint32_t parity, uint64_t* alive) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (;;) {
+        #pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        const uint64_t since = max(t0, *reinterpret_cast<volatile uint64_t*>(alive));
+        if (global_timer_ns() - since > kWaitLimitNs) {
+            *reinterpret_cast<volatile uint64_t*>(alive) = ~0ull;
             return false;
         }
     }
