@@ -637,7 +637,7 @@ def prefill_packed(Q, K, V, q_offsets, k_offsets=None, causal: bool = True, scal
     (fp16 or bf16, any 8-element aligned strides); sequence b has the rows q_offsets[b] .. q_offsets[b + 1] of Q and
     k_offsets[b] .. k_offsets[b + 1] of K and V (int32 CUDA tensors of batch + 1 entries; default: the same rows).  Causal: a sequence's
     last query sees all its keys, each one before it sees one key less, so keys beyond the queries are a cache in front of them.  A
-    query without keys gets zeros; rows of out outside all sequences are left as they are.  scale 0: 1 / sqrt(D)."""
+    query without keys gets zeros; rows of out outside all sequences are left as they are.  out overlaps no input.  scale 0: 1 / sqrt(D)."""
     if k_offsets is None:
         k_offsets = q_offsets
     if out is None:
@@ -698,7 +698,7 @@ def decode_shared(q, K_prefix, V_prefix, K, V, lengths, prefix_len=None, scale: 
     """One new token per sequence, behind a prefix that all sequences share and that is read once for all of them: q [batch, heads, D]
     attends to the first prefix_len keys of K_prefix / V_prefix [kv_heads, max_prefix, D] (default: all) and to the first lengths[b]
     keys of its own cache K / V [batch, kv_heads, max_own, D].  lengths: int32 CUDA tensor, read on the device.  A sequence without
-    keys gets zeros.  scale 0: 1 / sqrt(D)."""
+    keys gets zeros.  out overlaps no input.  scale 0: 1 / sqrt(D)."""
     if out is None:
         out = q.new_empty(q.shape)
     device = _together(q, (K_prefix, V_prefix, K, V, out), (lengths,))

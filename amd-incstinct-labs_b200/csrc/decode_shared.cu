@@ -156,6 +156,7 @@ template <typename T, int D, int NT> struct KeyWalk {
                 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) { o[n][i][0] *= alpha[0]; o[n][i][1] *= alpha[1]; o[n][i][2] *= alpha[0]; o[n][i][3] *= alpha[1]; }
             }
+            // in 16 bits, as V is: half a step of each weight (prefill_tc.cuh); l has added them in fp32
             pt[n][0] = transposed_8x8(pack2<T>(s[n][0], s[n][1])); pt[n][1] = transposed_8x8(pack2<T>(s[n][2], s[n][3]));
         }
         #pragma unroll
@@ -375,7 +376,9 @@ SharedPlan plan_shared(const b200p_shared_args& a) {
         // and merge, which saves a launch (99 sequences, 2423 + up to 441 keys, 6 / 2 heads of 64, 14.9 -> 13.5 us; 145, 2984 + up to 306, 2 / 1,
         // 11.5 -> 9.9).  CTAs that wait where there is no room hold the SMs that others could begin on (48 of 32 / 4 heads of 64, 5000 + up to 1000,
         // 19.2 -> 26.4; 256, 32768 + up to 256, 32 / 8 of 128, 141 -> 157); short caches of heads of 64 are read soon enough all the same (103,
-        // 4127 + up to 140, 16 / 4, 18.4 -> 16.1).  Many parts are quicker in merge_kernel's many warps (2 sequences, 14997 + up to 191, 16 / 4 of 128, 15.2 against 16.8).
+        // 4127 + up to 140, 16 / 4, 18.4 -> 16.1).  Many parts are quicker in merge_kernel's many warps. A unit's CTAs read group * splits * D
+        // fp32 values of them, joined and apart: 5120 21.6 and 22.0 us (8 sequences, 12000 + up to 100 keys, 4 / 1 of 128), 12288 14.0 and 13.8 (4, 8000 + up to 100, 8 / 2),
+        // 16384 22.8 and 18.9 (2, 15000 + up to 100, 8 / 1), 31744 18.2 and 14.0; below 6500 some lose too (16, 9000 + up to 100, 8 / 1, 6144: 29.0 and 25.9), above some gain 0.8.
         const long long items = (long long)((tiles + span - 1) / span) * a.nKVHeads * splits;
         const long long room = (a.D == 64 && a.max_own <= 160 ? sms : sms - items) * (pl.rows == 8 ? 4 : a.D == 64 ? 3 : 2);
         int c = pl.cluster;

@@ -17,7 +17,9 @@ namespace {
 // In how many splits the keys are taken: for few query tiles with many keys (a few new tokens on a long cache), and for a few sequences
 // of which some may be much longer than the others.  The lengths are on the device, so the times, in microseconds, go by the means: an
 // item takes 3 and 1.35 per 128 keys (2.05 with two query tiles); the last one to end may be of a sequence 1.8 times as long and begins
-// when the others are under way; the merge takes 3, and the parts' way through the workspace.  A split has two key tiles at least.
+// when the others are under way; the merge takes 3, and the parts' way through the workspace.  A split has two
+// key tiles, by the mean of the sequences' keys, but for what the last one is left with (a mean of 300 keys may take two); a shorter sequence leaves
+// splits without keys.
 // (One and the number chosen, 8 / 2 heads of 128: 39 tokens each of 11 sequences on 3950 keys 81 and 30; 2 texts of 1000 and 5000 tokens, one head, 72 and 28;
 // 32 / 8 heads: 4 times 16 tokens on 1500 keys 32.6 and 18; 300 tokens, 300 keys, 10.3 and, with 2, 11.4: none.  Of 280 drawn calls of 200 keys and
 // more the mean is 4 % above the best number of splits tried; the worst, 1.65 times, where one sequence has most of the tokens.)

@@ -200,3 +200,10 @@ def test_rules_set_just_ahead_of_a_call_on_another_stream(b200p, torch_cuda):
                 s.set_rules(allowed=[t], presence=0.5)
             assert (s.generate(ids, 2)[0] == t).all()
     s.close()
+
+
+def test_generate_program_with_nothing_allowed(torch_cuda):
+    model = os.path.join(ROOT, "tests", "golden", "tiny_llama")
+    for rules in (["--allow", ""], ["--allow", "7 8", "--ban", "8 7"]):
+        r = subprocess.run([os.path.join(ROOT, "bin", "generate"), "--model", model, "--max-new", "4", "--prompt", "1 2 3 4", *rules], capture_output=True, text=True, timeout=300)
+        assert r.returncode != 0 and not r.stdout.split(), r.stdout
